@@ -197,6 +197,85 @@ int q3_linear_tc(const void* w, const float* x, float* out, const float* resid, 
 int q3_sample(const float* logits, int32_t batch, int32_t vocab, float temperature, int32_t top_k,
               const float* uniform, int64_t* out_tokens, void* stream);
 
+/* ---- a pool of cache pages -------------------------------------------------------------------------------------------
+ * Many sequences whose K and V rows live in pages of `page_size` positions, in any order, each sequence with a row of a
+ * page table: position p of sequence b is slot p % page_size of page page_table[b][p / page_size].  An entry outside
+ * 0 .. n_pages - 1 is a page that is not there: nothing is written to it, its positions are not attended.  The new tokens of a call
+ * are rows of q, k and v, sequence after sequence: sequence b's are rows q_start[b] .. q_start[b + 1] - 1 and its last
+ * kv_len[b] - (kv_len[b] - new) positions, i.e. its token i stands at position kv_len[b] - new + i.  A sequence may have no new token; rows
+ * behind q_start[batch] belong to nobody and are left as they were.  All descriptors lie in device memory and are read
+ * when the call runs: a captured call may be replayed with others.  What they say is cut down to what there is
+ * (n_tokens rows, table_pages * page_size positions), so that no value reads or writes out of bounds.
+ * Strides are in elements; the 128 elements of a head are contiguous, pages 16-byte aligned and strides multiples of 8, the same for K and V. */
+#define Q3_TYPE_BF16 0
+#define Q3_TYPE_FP16 1
+#define Q3_TYPE_FP32 2   /* rows of q3_paged_rope only */
+#define Q3_PAGED_MAX_BATCH 1024
+typedef struct q3_paged {
+    void* k_pages;               /* device: element (page, slot, head, dim) at page * page_stride + slot * slot_stride + head * head_stride + dim */
+    void* v_pages;
+    const int32_t* page_table;   /* device [batch][table_stride], table_pages entries a row */
+    const int32_t* q_start;      /* device [batch + 1], ascending                     */
+    const int32_t* kv_len;       /* device [batch]: positions with the new tokens     */
+    int64_t page_stride, slot_stride, head_stride;
+    int64_t table_stride;
+    int32_t table_pages;
+    int32_t n_pages;
+    int32_t page_size;           /* 16, 32, 64, 128 or 256                            */
+    int32_t batch;               /* 1 .. Q3_PAGED_MAX_BATCH                           */
+    int32_t n_tokens;            /* rows of q, k, v and out                           */
+    int32_t max_new;             /* most new tokens of a sequence, as the host knows it: chooses the kernel, bounds nothing */
+    int32_t kv_heads;            /* head dim is 128                                   */
+    int32_t type;                /* Q3_TYPE_BF16 or Q3_TYPE_FP16: pages, q, out of the attention */
+} q3_paged;
+
+/* Attention of the new tokens over their sequences' pages: out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the
+ * positions j of t's sequence up to t's own (the new tokens' k and v rows are in the pages, see q3_paged_rope).  q_heads is
+ * kv_heads times 1, 2, 4 or 8; q head h reads kv head h / (q_heads / kv_heads).  A token that sees no position, or none with a weight (all
+ * scores -inf), gets zeros; a row that it does not see does not touch its result, whatever it holds.  fp32 scores, maxima, sums and
+ * accumulators; the probabilities enter the product with V in the pages' type.  q and out: element (token, head, dim) at token * _token + head * _head + dim, 16-byte
+ * aligned, strides multiples of 8.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
+ * `status`: device, 4 words, or NULL: a wait inside the kernel that gives up reports there as in q3_status and leaves NaN in the rows
+ * it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
+typedef struct q3_paged_attn_args {
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, out_token, out_head;
+    int32_t q_heads;
+    float scale;                 /* > 0, at most 1e30, usually 128^-0.5 */
+    void* workspace;
+    int64_t workspace_bytes;
+    uint32_t* status;
+} q3_paged_attn_args;
+int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads);   /* bytes; depends on the device and the head counts alone, negative: an error code */
+int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* a, void* stream);
+
+/* The new tokens' q, k and v rows on their way to that attention: RMS norm of every q and k head (where a gain is given), rotary embedding of its
+ * first rotary_dim dims by the table row of the token's position, and the k and v rows rounded once into the slots of their pages:
+ *     n = x rsqrt(mean(x^2) + eps) gain
+ *     half layout:  y[i] = n[i] c[i] - n[i + r/2] s[i],   y[i + r/2] = n[i + r/2] c[i] + n[i] s[i],      i < r/2 = rotary_dim / 2
+ *     interleaved:  y[2i] = n[2i] c[i] - n[2i + 1] s[i],  y[2i + 1] = n[2i + 1] c[i] + n[2i] s[i]
+ * in fp32.  q, k and v: element (token, head, dim) at token * _token + head * _head + dim (they may be slices of one row), 16-byte aligned fp32 or 8-byte
+ * aligned bf16 / fp16, strides multiples of 4; q_out as q_paged_attn's q.  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
+ * rotary_dim / 2 angles (any scaling of long contexts is in the table).  A token whose position has no row gets NaN (q, k); one without a slot (no page, or
+ * kv_len below the number of new tokens) writes no k and v.  `positions`: device [n_tokens] or NULL: rotate by these instead of the tokens' places
+ * in their sequences.  q may be NULL (k and v only), and k and v both (q only).  Allocates nothing, no host sync. */
+typedef struct q3_paged_rope_args {
+    const void *q, *k, *v;
+    void* q_out;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    const void *q_gain, *k_gain; /* device bf16 [128] or NULL: no norm */
+    const float* rope;           /* device; NULL when rotary_dim is 0  */
+    const int32_t* positions;
+    int32_t q_heads;
+    int32_t rows_type;           /* Q3_TYPE_* of q, k and v            */
+    int32_t rope_positions;
+    int32_t rotary_dim;          /* a multiple of 8, 0 .. 128          */
+    int32_t interleaved;
+    float eps;
+} q3_paged_rope_args;
+int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* a, void* stream);
+
 /* Synchronise `stream`, read the device status words and clear them.  Returns Q3_OK or
  * Q3_ERR_DEVICE_WAIT; `words` (may be NULL) receives up to `n` raw status words:
  * [0] error code, [1] where (phase id), [2] CTA index, [3] observed counter value. */

@@ -10,7 +10,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_NOT_RESIDENT, ERR_DEVICE_WAIT, ERR_UNSUPPORTED = 
 F_APPEND_KV, F_PATH_AUTO, F_PATH_LAYERED, F_PATH_PERSIST, F_PATH_FUSED, F_GRAPH = 0x1, 0x0, 0x10, 0x20, 0x30, 0x100
 
 # every symbol include/q3mk.h declares
-SYMBOLS = ("q3_create", "q3_destroy", "q3_set_weights", "q3_invalidate_weights", "q3_set_rope", "q3_tp_export", "q3_tp_attach", "q3_decode", "q3_decode_noalloc", "q3_noalloc_status", "q3_linear_tc", "q3_prefill", "q3_sample", "q3_status",
+SYMBOLS = ("q3_create", "q3_destroy", "q3_set_weights", "q3_invalidate_weights", "q3_set_rope", "q3_tp_export", "q3_tp_attach", "q3_decode", "q3_decode_noalloc", "q3_noalloc_status", "q3_linear_tc", "q3_prefill", "q3_sample", "q3_paged_attn_workspace", "q3_paged_attn", "q3_paged_rope", "q3_status",
            "q3_set_trace", "q3_launch_count", "q3_grid_info", "q3_scratch", "q3_last_error", "q3_version")
 
 WEIGHT_FIELDS = ("ln1", "wq", "wk", "wv", "qn", "kn", "wo", "ln2", "wg", "wu", "wd", "fnorm", "embed")
@@ -35,6 +35,26 @@ class DecodeArgs(C.Structure):
 class PrefillArgs(C.Structure):
     _fields_ = [("n_tokens", C.c_int32), ("cache_capacity", C.c_int32), ("ids", C.c_void_p), ("kcache", C.c_void_p),
                 ("vcache", C.c_void_p), ("last_logits", C.c_void_p), ("next_token", C.c_void_p)]
+
+
+class Paged(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_table", C.c_void_p), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_stride", C.c_int64), ("slot_stride", C.c_int64), ("head_stride", C.c_int64), ("table_stride", C.c_int64),
+                ("table_pages", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("batch", C.c_int32),
+                ("n_tokens", C.c_int32), ("max_new", C.c_int32), ("kv_heads", C.c_int32), ("type", C.c_int32)]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_token", C.c_int64), ("q_head", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64),
+                ("q_heads", C.c_int32), ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p)]
+
+
+class PagedRopeArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64), ("v_token", C.c_int64), ("v_head", C.c_int64),
+                ("out_token", C.c_int64), ("out_head", C.c_int64), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("rope", C.c_void_p),
+                ("positions", C.c_void_p), ("q_heads", C.c_int32), ("rows_type", C.c_int32), ("rope_positions", C.c_int32), ("rotary_dim", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float)]
 
 
 _lib = None
@@ -76,6 +96,12 @@ def load() -> C.CDLL:
     lib.q3_prefill.restype = C.c_int
     lib.q3_sample.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.q3_sample.restype = C.c_int
+    lib.q3_paged_attn_workspace.argtypes = [C.POINTER(Paged), C.c_int32]
+    lib.q3_paged_attn_workspace.restype = C.c_int64
+    lib.q3_paged_attn.argtypes = [C.POINTER(Paged), C.POINTER(PagedAttnArgs), C.c_void_p]
+    lib.q3_paged_attn.restype = C.c_int
+    lib.q3_paged_rope.argtypes = [C.POINTER(Paged), C.POINTER(PagedRopeArgs), C.c_void_p]
+    lib.q3_paged_rope.restype = C.c_int
     lib.q3_status.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint32), C.c_int32]
     lib.q3_status.restype = C.c_int
     lib.q3_set_trace.argtypes = [C.c_void_p, C.c_void_p, C.c_int64]
