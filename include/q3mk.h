@@ -197,6 +197,32 @@ int q3_linear_tc(const void* w, const float* x, float* out, const float* resid, 
 int q3_sample(const float* logits, int32_t batch, int32_t vocab, float temperature, int32_t top_k,
               const float* uniform, int64_t* out_tokens, void* stream);
 
+/* Sample one token per row with parameters of the row's own: weights w = exp((logit - max) / temperature); keep the top_k largest logits (0 or at least
+ * vocab = all; ties at the k-th value are all kept); of these the most likely words until their weights reach top_p times the sum of the
+ * kept ones (equal words: the lowest index first; 1 or more = all, 0 = the first); of these the words with w >= min_p (0 = all; the most
+ * likely word is always kept); return the first index whose inclusive sum of kept weights exceeds uniform[row] * total, in index order.  The
+ * arrays (device, [batch]) may be NULL: then the number beside them serves all rows.  temperature <= 0, top_k == 1 or min_p > 1, and rows that have no draw (a NaN
+ * or an infinite maximum among the logits, a uniform number outside [0, 1)) give the arg-max (ties -> lowest index).  Logits of -inf are never
+ * drawn; values that no parameter may have (a NaN, a negative top_k) switch that filter off, a temperature that is NaN gives the arg-max.  Row r begins at logits + r * row_stride.  The same
+ * logits and numbers draw the same words on every run.  Allocates nothing, no host sync.  q3_sample, with one temperature and one top_k for all rows, sums in fp32. */
+typedef struct q3_sample_rows_args {
+    const float* logits;         /* device [batch][row_stride] fp32, vocab words a row */
+    int64_t row_stride;          /* >= vocab, or 0: many draws from one row            */
+    const float* temperatures;   /* device [batch] or NULL                             */
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    const float* uniform;        /* device [batch], in [0, 1)                          */
+    int64_t* out_tokens;         /* device [batch]                                     */
+    int32_t batch;               /* 1 .. 2^20                                          */
+    int32_t vocab;               /* 1 .. 2^22                                          */
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+} q3_sample_rows_args;
+int q3_sample_rows(const q3_sample_rows_args* a, void* stream);
+
 /* ---- a pool of cache pages -------------------------------------------------------------------------------------------
  * Many sequences whose K and V rows live in pages of `page_size` positions, in any order, each sequence with a row of a
  * page table: position p of sequence b is slot p % page_size of page page_table[b][p / page_size].  An entry outside

@@ -1,4 +1,5 @@
-"""Temperature / top-k sampling on the GPU over the fp32 logits of a decode step.
+"""Sampling on the GPU over the fp32 logits of a decode step: `sample` with one temperature and top-k, `sample_rows` with a temperature, top-k, top-p and
+min-p of its own for every row.
 
 The reference decodes greedily and returns the fp32 logits "for the caller" (qwen3mk/kernel.py:44-50); this module is
 the step after that: `sample` picks one token per row through the C ABI (`q3_sample`), with the uniform numbers drawn
@@ -7,6 +8,9 @@ reads.  `sample_reference` states the same rule in plain PyTorch on whatever dev
 documentation of the rule, not a fallback (`sample` fails without the CUDA library).
 """
 from __future__ import annotations
+
+import contextlib
+import ctypes
 
 import torch
 
@@ -51,3 +55,43 @@ def sample_reference(logits: torch.Tensor, temperature: float, top_k: int, u: to
     cdf = w.cumsum(dim=-1)
     target = u.reshape(-1, 1).double().to(rows.device) * cdf[:, -1:]
     return (cdf > target).double().argmax(dim=-1).reshape(logits.shape[:-1])
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def sample_rows(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, u: torch.Tensor | None = None, generator: torch.Generator | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of `logits` (CUDA fp32 [batch, vocab], contiguous words, any row stride), each filter a number or a CUDA tensor [batch] (float32; top_k int32).
+
+    A row keeps its top_k largest logits (0: all; ties are all kept), of these the most likely words until their weights exp((l - max) / temperature) reach top_p of their sum
+    (equal words: the lowest index first), of these the words of at least min_p times the most likely one's weight; the token is the first index whose cumulative weight
+    exceeds u times the total.  temperature <= 0, top_k = 1, top_p = 0 or min_p > 1: the arg-max.  `u` (CUDA fp32 [batch], in [0, 1)) overrides the generator.
+    Enqueues on the current stream of the logits' device and returns the int64 tokens [batch] (`out` when given) without synchronising; equal inputs draw equal words."""
+    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[0] < 1 or (logits.shape[1] != 1 and logits.stride(1) != 1):
+        raise ValueError("sample_rows: logits must be a CUDA float32 tensor [batch, vocab] with contiguous words")
+    batch, vocab, dev = logits.shape[0], logits.shape[1], logits.device
+    ptrs, values = [], []
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(x, torch.Tensor):
+            if x.dtype != dtype or x.shape != (batch,) or x.device != dev or not x.is_contiguous():
+                raise ValueError(f"sample_rows: {name} must be a number or a contiguous {dtype} tensor [{batch}] on {dev}")
+            ptrs.append(x.data_ptr()), values.append(0)
+        else:
+            ptrs.append(None), values.append(x)
+    if u is None:
+        u = torch.rand(batch, device=dev, dtype=torch.float32, generator=generator)
+    elif u.dtype != torch.float32 or u.shape != (batch,) or u.device != dev or not u.is_contiguous():
+        raise ValueError(f"sample_rows: u must be a contiguous float32 tensor [{batch}] on {dev}")
+    if out is None:
+        out = torch.empty(batch, dtype=torch.int64, device=dev)
+    elif out.dtype != torch.int64 or out.shape != (batch,) or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"sample_rows: out must be a contiguous int64 tensor [{batch}] on {dev}")
+    lib = _cabi.load()
+    a = _cabi.SampleRowsArgs(logits.data_ptr(), logits.stride(0) if batch > 1 else vocab, *ptrs, u.data_ptr(), out.data_ptr(), batch, vocab, float(values[0]), int(values[1]),
+                             float(values[2]), float(values[3]))
+    with _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
+        rc = lib.q3_sample_rows(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _cabi.check(lib, None, rc, "q3_sample_rows")
+    return out
