@@ -232,7 +232,8 @@ int q3_sample_rows(const q3_sample_rows_args* a, void* stream);
  * behind q_start[batch] belong to nobody and are left as they were.  All descriptors lie in device memory and are read
  * when the call runs: a captured call may be replayed with others.  What they say is cut down to what there is
  * (n_tokens rows, table_pages * page_size positions), so that no value reads or writes out of bounds.
- * Strides are in elements; the 128 elements of a head are contiguous, pages 16-byte aligned and strides multiples of 8, the same for K and V. */
+ * Strides are in elements; the 128 elements of a head are contiguous, pages 16-byte aligned and strides multiples of 8 that are at
+ * least 128, the same for K and V. */
 #define Q3_TYPE_BF16 0
 #define Q3_TYPE_FP16 1
 #define Q3_TYPE_FP32 2   /* rows of q3_paged_rope only */
@@ -260,7 +261,7 @@ typedef struct q3_paged {
  * kv_heads times 1, 2, 4 or 8; q head h reads kv head h / (q_heads / kv_heads).  A token that sees no position, or none with a weight (all
  * scores -inf), gets zeros; a row that it does not see does not touch its result, whatever it holds.  fp32 scores, maxima, sums and
  * accumulators; the probabilities enter the product with V in the pages' type.  q and out: element (token, head, dim) at token * _token + head * _head + dim, 16-byte
- * aligned, strides multiples of 8.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
+ * aligned, strides multiples of 8, at least 128.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
  * `status`: device, 4 words, or NULL: a wait inside the kernel that gives up reports there as in q3_status and leaves NaN in the rows
  * it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
 typedef struct q3_paged_attn_args {
@@ -273,7 +274,7 @@ typedef struct q3_paged_attn_args {
     int64_t workspace_bytes;
     uint32_t* status;
 } q3_paged_attn_args;
-int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads);   /* bytes; depends on the device and the head counts alone, negative: an error code */
+int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads);   /* bytes; depends on the device, the head counts and max_new alone, negative: an error code */
 int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* a, void* stream);
 
 /* The new tokens' q, k and v rows on their way to that attention: RMS norm of every q and k head (where a gain is given), rotary embedding of its

@@ -8,6 +8,7 @@
 #include <cfloat>
 
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 
 #include "q3_engine.h"
@@ -368,6 +369,455 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
+// Chunks of new tokens: 128 rows (128 / group tokens of every q head of a kv head) against tiles of 128 keys on tcgen05.mma, accumulators in TMEM.
+//     S  = Q K^T     M 128 x N 128 keys x K 128 dims, both K-major        -> TMEM columns [0, 128) / [128, 256), by the parity of the tile
+//     P  = 2^(S - m) two groups of eight warps, two threads a row (64 keys each); group g takes the tiles of parity g, so that one group's exponentials
+//                    run while the tensor pipe and the hand-offs of the other's tile do.  P takes the place of S in TMEM
+//     O += P V       V is the MN-major operand straight from its tile; an O a group -> columns [256, 384) / [384, 512)
+// as in q3_prefill_attn_tc.cu, and beyond it: K and V come page by page (a TMA box a page and half of the dims; a page that is not there, or that no row of the tile sees, lies
+// outside the tensor and reads as zeros), and a block walks the segments of its run without draining: tiles are counted over all of them, the next segment's Q
+// has a buffer of its own, its first scores are under way while the last one's rows are finished.
+// O is rescaled only when a score exceeds the maximum that P is taken under by 2^8.
+// A wait that gives up lets every later one give up at once; all warps still meet at every barrier, rows that are not finished become NaN, and the block drains
+// what is under way before it leaves.
+// ------------------------------------------------------------------------------------------------------------------------------
+constexpr int PT_SOFT = 512, PT_THREADS = PT_SOFT + 64;       // warps 0..15 softmax and output, 16 TMA, 17 MMA and TMEM
+constexpr int PT_KEYS = 128;                                  // keys of a tile, the unit of work
+constexpr uint32_t PT_BOX = 128 * 128, PT_TILE = 2 * PT_BOX;  // [128 rows][64 dims] with 128-byte swizzle; 128 x 128
+constexpr size_t PT_SMEM = 2 * PT_TILE + 2 * 2 * PT_TILE;     // two of Q, two stages of K and V
+constexpr float PT_LAG = 8.f;
+
+// The thread looks at the barrier without being parked: a tile has eight hand-offs.
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
+    unsigned it = 0;
+    unsigned long long t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        if ((++it & 63u) == 0) {
+            const unsigned long long t = tc_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > TC_WAIT_NS) {
+                if (status) report(status, ST_MBAR_TIMEOUT, site, parity);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool pt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
+    return one_lane_waits([&] { return pt_wait(bar, parity, abort_flag, status, site); });
+}
+// MN-major operand: rows are keys (the K index), 64 dims a row; the next 64 dims a box further, the next 8 keys 1024 bytes
+__device__ __forceinline__ uint64_t pt_desc_mn(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (uint64_t)(PT_BOX >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pt_init(uint64_t* bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(bar)), "r"(count) : "memory"); }
+__device__ __forceinline__ void pt_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void pt_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(tc_smem(bar)) : "memory"); }
+__device__ __forceinline__ void pt_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc_smem(bar)) : "memory");
+}
+__device__ __forceinline__ int pt_tiles(const PgKeys& k) { return (k.key1 - k.key0 + PT_KEYS - 1) / PT_KEYS; }
+
+template <typename T>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                                                                   const __grid_constant__ CUtensorMap tm_v, const PagedAttnArgs a) {
+    extern __shared__ __align__(1024) unsigned char pt_raw[];
+    __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PT_THREADS / 32];
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free, drain_bar;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ volatile int abort_flag;
+    __shared__ float s_max[2][2][2][128];           // per group and parity of its tiles: the tile's maximum of a row's two halves
+    __shared__ float s_m[2][128], s_l[2][2][128];   // at a segment's end: per group, a row's maximum and the two halves of its sum
+    __shared__ unsigned s_bad[4];
+    __shared__ float s_res[132];
+
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
+    pdl_launch();
+    pdl_wait();
+    pg_block_prefix<PT_THREADS>(a.sh, a.c.q_start, a.c.kv_len, s_prefix, s_sum);
+    const long long total = s_prefix[a.sh.batch];
+    const int blocks = pg_blocks(total, (int)gridDim.x, a.least);
+    if ((int)blockIdx.x >= blocks) return;
+    unsigned char* const sKV = pt_raw + 2 * PT_TILE;  // stage s: K at s * 2 * PT_TILE, V right behind it
+    if (tid == 0) {
+        for (int s = 0; s < 2; ++s) {
+            pt_init(&k_full[s], 1); pt_init(&v_full[s], 1); pt_init(&k_empty[s], 1); pt_init(&v_empty[s], 1);
+            pt_init(&q_full[s], 1); pt_init(&q_empty[s], PT_SOFT / 32);
+            pt_init(&s_full[s], 1); pt_init(&p_full[s], 8); pt_init(&o_full[s], 1);
+        }
+        pt_init(&o_free, PT_SOFT / 32);
+        pt_init(&drain_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        abort_flag = 0;
+        s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
+    }
+    if (warp == PT_SOFT / 32 + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_base_s;
+    const int *qs = a.c.q_start, *kl = a.c.kv_len;
+    const long long from = pg_run_start(total, blocks, blockIdx.x), to = pg_run_start(total, blocks, blockIdx.x + 1);
+
+    int armed_k = 0, armed_v = 0, armed_q = 0;      // what the producer has requested
+    if (warp == PT_SOFT / 32) {
+        // ---------------------------------------------------------------------- TMA: a lane a box
+        const int rows_log = min(a.c.page_log, 7), boxes = PT_KEYS >> rows_log, j = lane >> 1, half = lane & 1;      // a page's rows are cut into boxes of 128 at most
+        const bool mine = j < boxes;
+        PgWalk w;
+        bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
+        int g = 0, n_q = 0;
+        while (ok) {
+            const PgKeys k = pg_keys(a, w.s);
+            const int n = pt_tiles(k);
+            auto page_of = [&](int t) {               // of this lane's box of tile t; n_pages: no such page, zeros
+                const int key = k.key0 + t * PT_KEYS + (j << rows_log);
+                if (!mine || key >= k.key1) return a.c.n_pages;
+                const int p = pg_page(a.c, w.s.b, key);
+                return p < 0 ? a.c.n_pages : p;
+            };
+            int page = n > 0 ? page_of(0) : 0;
+            if (n > 0) {
+                const int buf = n_q & 1;
+                if (n_q >= 2 && !pt_wait_warp(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) break;
+                if (lane == 0) {
+                    pt_expect(&q_full[buf], PT_TILE);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)       // rows past q are zeros
+                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                     ::"r"(tc_smem(pt_raw + buf * PT_TILE + b * PT_BOX)), "l"(&tm_q), "r"(64 * b), "r"(w.s.h * a.group), "r"(w.s.seq.q0 + w.s.r * a.sh.tile),
+                                       "r"(tc_smem(&q_full[buf])) : "memory");
+                }
+                armed_q = ++n_q;
+            }
+            for (int t = 0; t < n && ok; ++t, ++g) {
+                const int s = g & 1, slot = (k.key0 + t * PT_KEYS + (j << rows_log)) & ((1 << a.c.page_log) - 1);
+                const uint32_t dst = tc_smem(sKV + (size_t)s * 2 * PT_TILE) + (uint32_t)half * PT_BOX + ((uint32_t)j << (rows_log + 7));
+                const int next = t + 1 < n ? page_of(t + 1) : 0;
+                // K and V of a tile share a stage but are released separately: K as soon as the tile's scores are there
+                ok = g < 2 || pt_wait_warp(&k_empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
+                if (!ok) break;
+                if (lane == 0) pt_expect(&k_full[s], PT_TILE);
+                __syncwarp();
+                if (mine)
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                 ::"r"(dst), "l"(&tm_k), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&k_full[s])) : "memory");
+                armed_k = g + 1;
+                ok = g < 2 || pt_wait_warp(&v_empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 82);
+                if (!ok) break;
+                if (lane == 0) pt_expect(&v_full[s], PT_TILE);
+                __syncwarp();
+                if (mine)
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                 ::"r"(dst + PT_TILE), "l"(&tm_v), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&v_full[s])) : "memory");
+                armed_v = g + 1;
+                page = next;
+            }
+            ok = ok && w.next(a.sh, qs, kl);
+        }
+    } else if (warp == PT_SOFT / 32 + 1) {
+        // ---------------------------------------------------------------------- MMA issuer
+        if (elect_one()) {
+            const uint32_t idesc_s = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), idesc_o = idesc_s | (1u << 16);
+            constexpr uint64_t BOX = PT_BOX >> 4, TILE = PT_TILE >> 4;
+            const uint64_t dq = tc_desc(tc_smem(pt_raw)), dk = tc_desc(tc_smem(sKV)), dv = pt_desc_mn(tc_smem(sKV + PT_TILE));
+            // two walks over the same tiles: scores run two tiles ahead of the products with V
+            PgWalk ws, wp;
+            int gs = 0, ts = -1, ns = 0, q_s = -1;   // the tile whose scores come next: number, place in its segment, tiles of that, segments with tiles before it
+            auto next_s = [&]() -> bool {            // the next tile of ws, if there is one
+                if (ts + 1 < ns) { ++ts; return true; }
+                for (;;) {
+                    if (!(ts < 0 ? ws.begin(a.sh, s_prefix, qs, kl, from, to) : ws.next(a.sh, qs, kl))) return false;
+                    ns = pt_tiles(pg_keys(a, ws.s));
+                    ts = 0;
+                    if (ns > 0) { ++q_s; return true; }
+                }
+            };
+            auto issue_s = [&]() -> bool {
+                const int s = gs & 1, buf = q_s & 1;
+                if (ts == 0 && !pt_wait(&q_full[buf], (q_s >> 1) & 1, &abort_flag, a.status, 83)) return false;
+                if (!pt_wait(&k_full[s], (gs >> 1) & 1, &abort_flag, a.status, 84)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t dqs = dq + (uint64_t)buf * TILE, dks = dk + (uint64_t)s * 2 * TILE;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {        // 16 dims a step: four steps a box
+                    const uint64_t o = (uint64_t)(k >> 2) * BOX + (uint64_t)(k & 3) * 2;
+                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+                                 ::"r"(tmem_base + (uint32_t)s * 128u), "l"(dqs + o), "l"(dks + o), "r"(idesc_s), "r"(k ? 1u : 0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+                }
+                pt_commit(&s_full[s]);
+                pt_commit(&k_empty[s]);
+                ++gs;
+                return true;
+            };
+            bool more = next_s();
+            bool ok = true;
+            for (int i = 0; i < 2 && more && ok; ++i) {
+                ok = issue_s();
+                more = ok && next_s();
+            }
+            int g = 0, seg = 0;
+            bool left = ok && wp.begin(a.sh, s_prefix, qs, kl, from, to);
+            while (left && ok) {
+                const int n = pt_tiles(pg_keys(a, wp.s));
+                for (int t = 0; t < n && ok; ++t, ++g) {
+                    const int b = g & 1;
+                    if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
+                    ok = ok && pt_wait(&p_full[b], (g >> 1) & 1, &abort_flag, a.status, 86) && pt_wait(&v_full[b], (g >> 1) & 1, &abort_flag, a.status, 87);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t dvs = dv + (uint64_t)b * 2 * TILE;
+                    const uint32_t tp = tmem_base + (uint32_t)b * 128u;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)      // 16 keys a step: eight columns of P (two a column)
+                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+                                     ::"r"(tp + 256u), "r"(tp + (uint32_t)k * 8u), "l"(dvs + (uint64_t)k * (2048 >> 4)), "r"(idesc_o), "r"((t >= 2 || k) ? 1u : 0u),
+                                       "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+                    pt_commit(&o_full[b]);
+                    pt_commit(&v_empty[b]);
+                    if (more) {                      // over P of this tile: the pipe works in order
+                        ok = issue_s();
+                        more = ok && next_s();
+                    }
+                }
+                if (n > 0) ++seg;
+                left = wp.next(a.sh, qs, kl);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------------- softmax and output: row = TMEM lane
+        const int quad = warp & 3, row = quad * 32 + lane, grp = warp >> 3, part = (warp >> 2) & 1;   // part: 64 keys of a tile
+        const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
+        const uint32_t ts = trow + (uint32_t)(grp * 128), to_o = trow + 256u + (uint32_t)(grp * 128 + part * 64);
+        auto meet = [&] { asm volatile("bar.sync 9, %0;" ::"n"(PT_SOFT) : "memory"); };
+        PgWalk w;
+        bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
+        int g0 = 0, n_q = 0;
+        while (left) {
+            const PgKeys k = pg_keys(a, w.s);
+            const int n = pt_tiles(k);
+            const int last = min(k.qpos0 + row / a.group, k.key1 - 1);       // the last key this row sees
+            const bool live = quad * 32 < k.rows;                            // (the warp has a row)
+            const int t0 = (grp ^ g0) & 1;
+            float m = -INFINITY, lsum = 0.f;
+            auto pages_of = [&](int t) {             // bit i: whether keys 16 i .. of tile t have a page (or nobody sees them)
+                const int key = k.key0 + t * PT_KEYS + 16 * (lane & 7);
+                const bool there = t >= n || key >= k.key1 || pg_page(a.c, w.s.b, key) >= 0;
+                return there;
+            };
+            bool there = pages_of(t0);
+            for (int t = t0; t < n; t += 2) {
+                const int g = g0 + t, tile0 = k.key0 + t * PT_KEYS;
+                const uint32_t turn = (uint32_t)(g >> 1) & 1u;
+                const unsigned pages = __ballot_sync(0xffffffffu, there) & 0xffu;
+                there = pages_of(t + 2);
+                pt_wait_warp(&s_full[grp], turn, &abort_flag, a.status, 88);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (live) {
+                    uint32_t r[2][32];
+                    tc_ld32(r[0], ts + (uint32_t)(part * 64));
+                    tc_ld32(r[1], ts + (uint32_t)(part * 64 + 32));
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (tile0 + PT_KEYS - 1 > k.qpos0 || tile0 + PT_KEYS > k.key1 || pages != 0xffu) {
+                        const int key = tile0 + part * 64;
+                        const unsigned gone = ~(pages >> (part * 4));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            if (key + j > last || ((gone >> (j >> 4)) & 1u)) r[0][j] = 0xff800000u;            // -inf
+                            if (key + 32 + j > last || ((gone >> (2 + (j >> 4))) & 1u)) r[1][j] = 0xff800000u;
+                        }
+                    }
+                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) { x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[0][j])); x[2 + (j & 1)] = fmaxf(x[2 + (j & 1)], __uint_as_float(r[1][j])); }
+                    const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    // the row's other half is a thread of the warp four further; behind the barrier both have read their part of S, too
+                    s_max[grp][turn][part][row] = x0;
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + grp * 4 + quad) : "memory");
+                    const float top = fmaxf(x0, s_max[grp][turn][part ^ 1][row]) * a.scale;
+                    const bool raise = !(top <= m + PT_LAG);
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
+                        if (raise) m = top;
+                        lsum *= c;
+                        if (t >= 2) {                // O of the segment's tiles so far, once the last of them has been added
+                            pt_wait_warp(&o_full[grp], turn ^ 1u, &abort_flag, a.status, 89);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                            for (int h = 0; h < 64; h += 16) {
+                                uint32_t o[16];
+                                tc_ld16(o, to_o + (uint32_t)h);
+                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
+                                pt_st16(to_o + (uint32_t)h, o);
+                            }
+                        }
+                    }
+                    const float ms = m == -INFINITY ? 0.f : m;               // (nothing seen so far: every exponential is 0)
+                    float psum0 = 0.f, psum1 = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float e0 = pg_ex2(fmaf(__uint_as_float(r[h][2 * j]), a.scale, -ms)), e1 = pg_ex2(fmaf(__uint_as_float(r[h][2 * j + 1]), a.scale, -ms));
+                            psum0 += e0; psum1 += e1;
+                            pk[j] = T::pack(e0, e1);
+                        }
+                        pt_st16(ts + (uint32_t)(part * 32 + h * 16), pk);
+                    }
+                    lsum += psum0 + psum1;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                if (tile0 + PT_KEYS > k.key1) {
+                    // rows of V that no row of this tile sees but whose page is there: what they hold is not ours to multiply, even by 0
+                    const int rows_log = min(a.c.page_log, 7), z0 = k.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
+                    pt_wait_warp(&v_full[grp], turn, &abort_flag, a.status, 90);
+                    for (int i = tid & 255; i < (z1 - z0) * 16; i += 256)
+                        *reinterpret_cast<uint4*>(sKV + (size_t)grp * 2 * PT_TILE + PT_TILE + (size_t)((i >> 3) & 1) * PT_BOX + (size_t)(z0 + (i >> 4)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pt_arrive(&p_full[grp]);
+            }
+            // ---- the segment's rows ----
+            const int last_t = t0 < n ? t0 + (n - 1 - t0) / 2 * 2 : -1;      // this group's last tile
+            if (last_t >= 0) pt_wait_warp(&o_full[grp], (uint32_t)((g0 + last_t) >> 1) & 1u, &abort_flag, a.status, 91);
+            if (part == 0) s_m[grp][row] = m;
+            s_l[grp][part][row] = lsum;
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            meet();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float m0 = s_m[0][row], m1 = s_m[1][row], mx = fmaxf(m0, m1);
+            const float f0 = m0 == -INFINITY ? 0.f : m0 == mx ? 1.f : pg_ex2(m0 - mx), f1 = m1 == -INFINITY ? 0.f : m1 == mx ? 1.f : pg_ex2(m1 - mx);
+            float sum = (s_l[0][0][row] + s_l[0][1][row]) * f0 + (s_l[1][0][row] + s_l[1][1][row]) * f1;
+            const int dim0 = (warp >> 2) * 32;       // a quarter of the row's dims
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            if (n > 0 && live) {
+                uint32_t v[32];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float f = h ? f1 : f0;
+                    tc_ld32(v, trow + 256u + (uint32_t)(h * 128 + dim0));
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (f != 0.f)                    // (a group without a tile, or without a key that the row sees: TMEM may hold anything)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(v[j]), f, o[j]);
+                }
+            }
+            if (n > 0) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pt_arrive(&o_free);
+            }
+            const bool gave_up = abort_flag;
+            if (gave_up) sum = NAN;
+            bool bad = !(sum <= FLT_MAX);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) bad = bad || !(fabsf(o[j]) <= FLT_MAX);
+            if (bad && row < k.rows && !gave_up) atomicOr(&s_bad[quad], 1u << lane);
+            const bool whole = w.whole();
+            float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
+            const int buf = n_q & 1;
+            if (whole) {
+                const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                uint4 pk[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    pk[j] = make_uint4(T::pack(o[8 * j] * r, o[8 * j + 1] * r), T::pack(o[8 * j + 2] * r, o[8 * j + 3] * r), T::pack(o[8 * j + 4] * r, o[8 * j + 5] * r),
+                                       T::pack(o[8 * j + 6] * r, o[8 * j + 7] * r));
+                if (n > 0) {
+                    // through the place of Q (every product of the segment has completed), so that 16 lanes write a row's 256 bytes; 16-byte chunks XORed by the row
+                    uint4* const so = reinterpret_cast<uint4*>(pt_raw + buf * PT_TILE);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) so[row * 16 + ((dim0 / 8 + j) ^ (row & 7))] = pk[j];
+                } else if (row < k.rows) {           // nothing seen: zeros
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(pg_o_row(a, w.s, row) + dim0 * 2 + j * 16) = pk[j];
+                }
+            } else if (row < k.rows) {
+                float* const dst = parts + (size_t)row * PG_PART;
+                if (dim0 == 0) *reinterpret_cast<float2*>(dst) = make_float2(gave_up ? NAN : mx, sum);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(dst + 4 + dim0 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+            meet();
+            if (whole && n > 0) {
+                const uint4* const so = reinterpret_cast<const uint4*>(pt_raw + buf * PT_TILE);
+                for (int i = tid; i < k.rows * 16; i += PT_SOFT) {
+                    const int rr = i >> 4, c = i & 15;
+                    *reinterpret_cast<uint4*>(pg_o_row(a, w.s, rr) + c * 16) = so[rr * 16 + (c ^ (rr & 7))];
+                }
+            }
+            if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) {
+                meet();                              // (rows have been written, the buffer of Q is free)
+                for (int q = 0; q < 4; ++q)
+                    for (unsigned b = s_bad[q]; b; b &= b - 1) {
+                        const int rr = q * 32 + __ffs(b) - 1;
+                        pg_redo_row<T, PT_SOFT / 32>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 9);
+                        if (tid < 64) {
+                            const float L = s_res[1], r = L > 0.f || L != L ? 1.f / L : 0.f;
+                            if (whole) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, rr) + tid * 4) = T::pack(s_res[4 + 2 * tid] * r, s_res[5 + 2 * tid] * r);
+                            else {
+                                float* const dst = parts + (size_t)rr * PG_PART;
+                                dst[4 + 2 * tid] = s_res[4 + 2 * tid]; dst[5 + 2 * tid] = s_res[5 + 2 * tid];
+                                if (tid == 0) { dst[0] = s_res[0]; dst[1] = L; }
+                            }
+                        }
+                    }
+                meet();
+                if (tid < 4) s_bad[tid] = 0;
+            }
+            if (n > 0) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) pt_arrive(&q_empty[buf]);
+                ++n_q;
+            }
+            g0 += n;
+            first = false;
+            left = w.next(a.sh, qs, kl);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    // After a wait gave up (nobody waits any more): the loads land and the products end before this block's memory and columns are somebody else's.
+    if (warp == PT_SOFT / 32 && abort_flag && lane == 0) {
+        for (int i = max(0, armed_q - 2); i < armed_q; ++i) tc_drain(&q_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, armed_k - 2); i < armed_k; ++i) tc_drain(&k_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, armed_v - 2); i < armed_v; ++i) tc_drain(&v_full[i & 1], (i >> 1) & 1);
+    }
+    if (warp == PT_SOFT / 32 + 1) {
+        if (abort_flag && elect_one()) {
+            pt_commit(&drain_bar);
+            tc_drain(&drain_bar, 0);
+        }
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------
 // Items that were cut: a block per cut, the one at an item's first cut puts the item together.  A warp a row, a lane four dims.
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int PJ_THREADS = 128;
@@ -424,24 +874,61 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-static int pg_blocks_of_device() { return 2 * tc_sm_count(); }
+// New tokens of a sequence up to which the products are the few-row kernel's: 32 rows with all q heads of a kv head.
+static bool pg_few(int max_new, int group) { return max_new * (long long)group <= 32; }
 
 template <typename T, int NB>
-static cudaError_t launch_rows(const PagedAttnArgs& a, int grid, cudaStream_t st) {
+static cudaError_t launch_rows(PagedAttnArgs& a, cudaStream_t st) {
+    a.sh.unit = PR_UNIT;
+    a.sh.tile = 8 * NB / a.group;
+    a.least = 1;
+    const int grid = 2 * tc_sm_count();
     cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PR_SMEM);
     if (e == cudaSuccess) e = launch_chain(paged_rows_kernel<T, NB>, dim3(grid), dim3(PR_THREADS), PR_SMEM, st, a);
-    if (e == cudaSuccess && grid > 1) e = launch_chain(paged_join_kernel<T>, dim3(grid - 1, 2 * NB), dim3(PJ_THREADS), 0, st, a, grid, 8 * NB);
+    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid - 1, 2 * NB), dim3(PJ_THREADS), 0, st, a, grid, 8 * NB);
+    return e;
+}
+
+// Tensor maps of q [tokens][heads][128] and of the pages [pages][heads][slots][128]: boxes of 64 dims, 128-byte swizzle
+static bool pg_make_map(CUtensorMap* m, bool bf, const void* p, int rank, const uint64_t* dims, const int64_t* strides, const uint32_t* box) {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;      // (a benign race between host threads: the same value is written)
+    if (!fn) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return false;
+        fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4];
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; }
+    for (int i = 1; i < rank; ++i) s[i - 1] = dims[i] > 1 ? strides[i - 1] : 256;      // (a dimension of one element has no stride)
+    return fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(p), d, s, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+static cudaError_t launch_tiles(PagedAttnArgs& a, int q_heads, cudaStream_t st) {
+    a.sh.unit = PT_KEYS;
+    a.sh.tile = 128 / a.group;
+    a.least = 1;
+    CUtensorMap q, k, v;
+    const uint64_t dq[3] = {HEAD_DIM, (uint64_t)q_heads, (uint64_t)a.sh.n_tokens}, dk[4] = {HEAD_DIM, 1ull << a.c.page_log, (uint64_t)a.sh.heads, (uint64_t)a.c.n_pages};
+    const int64_t sq[2] = {a.q_head, a.q_token}, sk[3] = {a.c.slot_bytes, a.c.head_bytes, a.c.page_bytes};
+    const uint32_t bq[3] = {64, (uint32_t)a.group, (uint32_t)a.sh.tile}, bk[4] = {64, 1u << (a.c.page_log < 7 ? a.c.page_log : 7), 1, 1};
+    if (!pg_make_map(&q, T::BF, a.q, 3, dq, sq, bq) || !pg_make_map(&k, T::BF, a.c.k, 4, dk, sk, bk) || !pg_make_map(&v, T::BF, a.c.v, 4, dk, sk, bk)) return cudaErrorInvalidValue;
+    const int grid = tc_sm_count();
+    cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM);
+    if (e == cudaSuccess) e = launch_chain(paged_tile_kernel<T>, dim3(grid), dim3(PT_THREADS), PT_SMEM, st, q, k, v, a);
+    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid - 1, 8), dim3(PJ_THREADS), 0, st, a, grid, 128);
     return e;
 }
 
 template <typename T>
-static cudaError_t launch_attn(PagedAttnArgs& a, int max_new, cudaStream_t st) {
-    const int cols = max_new > 32 / a.group ? 32 : max_new * a.group, nb = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    a.sh.unit = PR_UNIT;
-    a.sh.tile = 8 * nb / a.group;
-    a.least = 1;
-    const int grid = pg_blocks_of_device();
-    return nb == 1 ? launch_rows<T, 1>(a, grid, st) : nb == 2 ? launch_rows<T, 2>(a, grid, st) : launch_rows<T, 4>(a, grid, st);
+static cudaError_t launch_attn(PagedAttnArgs& a, int max_new, int q_heads, cudaStream_t st) {
+    if (!pg_few(max_new, a.group)) return launch_tiles<T>(a, q_heads, st);
+    const int cols = max_new * a.group;
+    return cols <= 8 ? launch_rows<T, 1>(a, st) : cols <= 16 ? launch_rows<T, 2>(a, st) : launch_rows<T, 4>(a, st);
 }
 
 int paged_check(const char* who, const q3_paged* c) {
@@ -457,8 +944,9 @@ int paged_check(const char* who, const q3_paged* c) {
     if (c->type != Q3_TYPE_BF16 && c->type != Q3_TYPE_FP16) return bad("pages are bf16 or fp16");
     if ((reinterpret_cast<uintptr_t>(c->k_pages) | reinterpret_cast<uintptr_t>(c->v_pages)) & 15) return bad("pages must be 16-byte aligned");
     const int64_t most = 1ll << 38;
-    for (int64_t s : {c->page_stride, c->slot_stride, c->head_stride})
-        if (s < 0 || s > most || s % 8) return bad("strides of the pages must be multiples of 8 elements, not negative");
+    const struct { int64_t stride; int32_t count; } dims[3] = {{c->page_stride, c->n_pages}, {c->slot_stride, c->page_size}, {c->head_stride, c->kv_heads}};
+    for (const auto& d : dims)
+        if (d.stride < 0 || d.stride > most || d.stride % 8 || (d.count > 1 && d.stride < HEAD_DIM)) return bad("strides of the pages must be multiples of 8 elements, at least 128");
     if ((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->q_start) | reinterpret_cast<uintptr_t>(c->kv_len)) & 3)
         return bad("page_table, q_start and kv_len must be 4-byte aligned");
     return Q3_OK;
@@ -480,12 +968,13 @@ PagedView paged_view(const q3_paged* c) {
 
 using namespace q3;
 
-// two partial results a block: at most 32 rows for every one of two blocks an SM
+// two partial results a block: 32 rows at most for each of two blocks an SM, or 128 for one
 extern "C" int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads) {
     if (!c || q_heads < 1) return engine_fail(nullptr, Q3_ERR_INVALID, "q3_paged_attn_workspace: bad argument");
     const int sms = tc_sm_count();
     if (sms < 1) return engine_fail(nullptr, Q3_ERR_CUDA, "q3_paged_attn_workspace: no CUDA device");
-    return (int64_t)2 * pg_blocks_of_device() * 32 * PG_PART * 4;
+    const int group = q_heads / (c->kv_heads < 1 ? 1 : c->kv_heads);
+    return (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 32 : 128) * PG_PART * 4;
 }
 
 extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, void* stream) {
@@ -501,8 +990,9 @@ extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, voi
     if (!(p->scale > 0.f) || p->scale > 1e30f) return bad("scale must be positive and at most 1e30");
     if ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out) | reinterpret_cast<uintptr_t>(p->workspace)) & 15) return bad("q, out and workspace must be 16-byte aligned");
     const int64_t most = 1ll << 38;
-    for (int64_t s : {p->q_token, p->q_head, p->out_token, p->out_head})
-        if (s < 0 || s > most || s % 8) return bad("strides of q and out must be multiples of 8 elements, not negative");
+    const struct { int64_t stride; int32_t count; } dims[4] = {{p->q_token, c->n_tokens}, {p->out_token, c->n_tokens}, {p->q_head, p->q_heads}, {p->out_head, p->q_heads}};
+    for (const auto& d : dims)
+        if (d.stride < 0 || d.stride > most || d.stride % 8 || (d.count > 1 && d.stride < HEAD_DIM)) return bad("strides of q and out must be multiples of 8 elements, at least 128");
     const int64_t need = q3_paged_attn_workspace(c, p->q_heads);
     if (need < 0) return (int)need;
     if (p->workspace_bytes < need) return engine_fail(nullptr, Q3_ERR_INVALID, "%s: workspace holds %lld bytes, %lld needed", who, (long long)p->workspace_bytes, (long long)need);
@@ -518,7 +1008,7 @@ extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, voi
     a.status = p->status;
     cudaStream_t st = (cudaStream_t)stream;
     const int max_new = c->max_new < 1 ? 1 : c->max_new;
-    const cudaError_t err = c->type == Q3_TYPE_BF16 ? launch_attn<PgBf16>(a, max_new, st) : launch_attn<PgFp16>(a, max_new, st);
+    const cudaError_t err = c->type == Q3_TYPE_BF16 ? launch_attn<PgBf16>(a, max_new, p->q_heads, st) : launch_attn<PgFp16>(a, max_new, p->q_heads, st);
     if (err != cudaSuccess) return engine_fail(nullptr, Q3_ERR_CUDA, "%s: %s", who, cudaGetErrorString(err));
     return Q3_OK;
 }
