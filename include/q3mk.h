@@ -303,6 +303,24 @@ typedef struct q3_paged_rope_args {
 } q3_paged_rope_args;
 int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* a, void* stream);
 
+/* New tokens of many sequences through the whole model over a pool of pages: prompts, chunks of prompts, known turns and single tokens side by side in one
+ * call.  `pages` describes layer 0 (8 kv heads, bf16; n_tokens up to the larger of the engine's max_tokens and max_batch, which must be at least 4; batch up to
+ * max_batch), layer l's pages lie l * layer_stride elements further.  The tokens' K and V rows are written into their slots; kv_len counts them already, so the
+ * caller adds a sequence's new tokens to kv_len before the call.  logits [batch][vocab] and next_token [batch] are those of every sequence's last new token (a
+ * sequence without one gets zeros).  Positions reach to the RoPE table's end; descriptors that say more than there is are cut down and reported by q3_status (code 5, site 1100).
+ * Activations enter the products rounded to bf16, as a prompt's do; up to 64 sequences the same call gives the same bits.  `workspace`: device, q3_paged_attn_workspace(pages, 16) bytes, for this call alone.
+ * No host sync, allocates nothing on the device.  A captured call may be replayed with other descriptors and tokens. */
+typedef struct q3_extend_args {
+    const q3_paged* pages;
+    int64_t layer_stride;
+    const int64_t* ids;          /* device [n_tokens]                 */
+    float* logits;               /* device [batch][vocab] fp32, or NULL */
+    int64_t* next_token;         /* device [batch]                    */
+    void* workspace;
+    int64_t workspace_bytes;
+} q3_extend_args;
+int q3_extend(q3_engine* e, const q3_extend_args* a, void* stream);
+
 /* Synchronise `stream`, read the device status words and clear them.  Returns Q3_OK or
  * Q3_ERR_DEVICE_WAIT; `words` (may be NULL) receives up to `n` raw status words:
  * [0] error code, [1] where (phase id), [2] CTA index, [3] observed counter value. */

@@ -66,10 +66,12 @@ __device__ __forceinline__ PrRope pr_rope(const PromptParams& p, int t, int d) {
     const float* row = p.rope + (size_t)t * HEAD_DIM + d;
     return PrRope{__ldg(reinterpret_cast<const float4*>(row)), __ldg(reinterpret_cast<const float4*>(row + 64))};
 }
+// whether a head of q/k/v gets its norm and RoPE here; not where the projections go out as they are (no cache rows)
+__device__ __forceinline__ bool pr_normed(const PromptParams& p, int col0) { return col0 < Q_DIM + KV_DIM && p.kc != nullptr; }
 // One half-row step of a finished q, k or v head: dims d .. d + 3 (lo) and 64 + d .. 64 + d + 3 (hi) of `col0`'s head (a multiple of 128
-// in q | k | v) of token t.  lo and hi are normalised except for the head's gain (v: final).
+// in q | k | v) of token t.  lo and hi are normalised except for the head's gain (v, and every head where there is no cache: final).
 __device__ __forceinline__ void pr_finish_head(const PromptParams& p, int col0, int t, int d, float4 lo, float4 hi, float4 glo, float4 ghi, const PrRope& r) {
-    if (col0 < Q_DIM + KV_DIM) {
+    if (pr_normed(p, col0)) {
         lo = pr_mul(lo, glo); hi = pr_mul(hi, ghi);
         const float4 c = r.c, s = r.s;
         const float4 a = make_float4(lo.x * c.x - hi.x * s.x, lo.y * c.y - hi.y * s.y, lo.z * c.z - hi.z * s.z, lo.w * c.w - hi.w * s.w);
@@ -80,7 +82,7 @@ __device__ __forceinline__ void pr_finish_head(const PromptParams& p, int col0, 
         float* o = p.qkv + (size_t)t * QKV_DIM + col0 + d;
         *reinterpret_cast<float4*>(o) = lo;
         *reinterpret_cast<float4*>(o + 64) = hi;
-        if (col0 < Q_DIM) return;
+        if (col0 < Q_DIM || p.kc == nullptr) return;
     }
     if (col0 < Q_DIM) {
         lo = pr_mul(lo, PR_QS); hi = pr_mul(hi, PR_QS);
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(PS_THREADS, OCC) prompt_split_kernel(const __g
         // (a thread per row all the way: prompts of 128 / 256 / 512 tokens 1002 / 1154 / 1550 us, so 975 / 1079 / 1437).
         constexpr int HALF = BN / 2, SUBS = BN / 8, STEP = 32 / SUBS, RB = SUBS < 8 ? SUBS : 8, LD = BN + 4;   // RB: rows whose RoPE entries are requested together
         const int col0 = tile * HEAD_DIM, d0 = rank * HALF, sub = lane % SUBS, lr0 = lane / SUBS, w0 = m0 + quad * 32, wrows = min(32, rows - quad * 32);
-        const bool normed = col0 < Q_DIM + KV_DIM;
+        const bool normed = pr_normed(p, col0);
         float* const piece = reinterpret_cast<float*>(base) + (size_t)quad * 32 * LD;
         static_assert(STAGES * S::STAGE >= 128 * LD * 4, "the stages hold the rows");
         PrRope rope[RB];
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prompt_pair_kernel(const __grid
                     for (int c = 0; c < 4; ++c) tc_ld32(v[c], tacc + (uint32_t)(half * 128 + c * 32));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     float f = r;
-                    if (col0 < Q_DIM + KV_DIM) {
+                    if (pr_normed(p, col0)) {
                         float ss[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int j = 0; j < 32; ++j)

@@ -26,7 +26,8 @@ struct PromptGemmCall {
     // PR_QKV: head norm, RoPE, then
     bf16_raw *q_hi, *q_lo;         // [T][2048] q times the softmax scale as two planes (read by the tiled attention), or
     float* qkv;                    // [T][4096] fp32 q, k, v rows (read by the split attention of few tokens)
-    bf16_raw *kc, *vc;             // this layer's cache rows [T..][1024]
+    bf16_raw *kc, *vc;             // this layer's cache rows [T..][1024]; both null: qkv holds the projections without head norm and RoPE (tokens of
+                                   // several sequences, q3_extend.cu; `rope` is then any T rows, nothing of them is used)
     const bf16_raw *qn, *kn;       // [128] head gains of this layer
     const float* rope;             // [positions][128], 16-byte aligned
     // PR_RESID

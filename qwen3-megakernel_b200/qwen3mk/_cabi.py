@@ -10,7 +10,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_NOT_RESIDENT, ERR_DEVICE_WAIT, ERR_UNSUPPORTED = 
 F_APPEND_KV, F_PATH_AUTO, F_PATH_LAYERED, F_PATH_PERSIST, F_PATH_FUSED, F_GRAPH = 0x1, 0x0, 0x10, 0x20, 0x30, 0x100
 
 # every symbol include/q3mk.h declares
-SYMBOLS = ("q3_create", "q3_destroy", "q3_set_weights", "q3_invalidate_weights", "q3_set_rope", "q3_tp_export", "q3_tp_attach", "q3_decode", "q3_decode_noalloc", "q3_noalloc_status", "q3_linear_tc", "q3_prefill", "q3_sample", "q3_sample_rows", "q3_paged_attn_workspace", "q3_paged_attn", "q3_paged_rope", "q3_status",
+SYMBOLS = ("q3_create", "q3_destroy", "q3_set_weights", "q3_invalidate_weights", "q3_set_rope", "q3_tp_export", "q3_tp_attach", "q3_decode", "q3_decode_noalloc", "q3_noalloc_status", "q3_linear_tc", "q3_prefill", "q3_sample", "q3_sample_rows", "q3_paged_attn_workspace", "q3_paged_attn", "q3_paged_rope", "q3_extend", "q3_status",
            "q3_set_trace", "q3_launch_count", "q3_grid_info", "q3_scratch", "q3_last_error", "q3_version")
 
 WEIGHT_FIELDS = ("ln1", "wq", "wk", "wv", "qn", "kn", "wo", "ln2", "wg", "wu", "wd", "fnorm", "embed")
@@ -55,6 +55,11 @@ class PagedRopeArgs(C.Structure):
                 ("out_token", C.c_int64), ("out_head", C.c_int64), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("rope", C.c_void_p),
                 ("positions", C.c_void_p), ("q_heads", C.c_int32), ("rows_type", C.c_int32), ("rope_positions", C.c_int32), ("rotary_dim", C.c_int32),
                 ("interleaved", C.c_int32), ("eps", C.c_float)]
+
+
+class ExtendArgs(C.Structure):
+    _fields_ = [("pages", C.POINTER(Paged)), ("layer_stride", C.c_int64), ("ids", C.c_void_p), ("logits", C.c_void_p), ("next_token", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 class SampleRowsArgs(C.Structure):
@@ -102,6 +107,8 @@ def load() -> C.CDLL:
     lib.q3_prefill.restype = C.c_int
     lib.q3_sample.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.q3_sample.restype = C.c_int
+    lib.q3_extend.argtypes = [C.c_void_p, C.POINTER(ExtendArgs), C.c_void_p]
+    lib.q3_extend.restype = C.c_int
     lib.q3_sample_rows.argtypes = [C.POINTER(SampleRowsArgs), C.c_void_p]
     lib.q3_sample_rows.restype = C.c_int
     lib.q3_paged_attn_workspace.argtypes = [C.POINTER(Paged), C.c_int32]

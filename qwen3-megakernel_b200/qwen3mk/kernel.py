@@ -223,6 +223,14 @@ class Megakernel:
         self.lib.q3_invalidate_weights(self.handle)
         self._weights_key = None
 
+    def set_rope(self, table: torch.Tensor) -> None:
+        """Rotary table of every later call: fp32 [positions, 128] on the engine's device (`paged.rope_table`, scaled for long contexts, say).  Borrowed; a bound
+        launch follows it with its next launch."""
+        if table.dim() != 2 or table.shape[1] != HEAD_DIM or table.dtype != torch.float32 or not table.is_contiguous() or table.device != self.device:
+            raise ValueError(f"set_rope: expected a contiguous float32 [positions, {HEAD_DIM}] on {self.device}, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        _cabi.check(self.lib, self.handle, self.lib.q3_set_rope(self.handle, table.data_ptr(), table.shape[0]), "q3_set_rope")
+        self.rope = table
+
     def check_inputs(self, inputs: dict) -> None:
         """Raise ValueError unless every input is a contiguous CUDA tensor of the expected shape and dtype."""
         ctx = inputs["kcache"].shape[1] if "kcache" in inputs and inputs["kcache"].dim() == 4 else CONTEXT
@@ -295,6 +303,29 @@ class Megakernel:
         self._decode(a, torch.cuda.current_stream(self.device).cuda_stream)
         self._next = self._alloc()
         return {"logits": logits, "next_token": next_token, "k_write": k_write, "v_write": v_write}
+
+    # ------------------------------------------------------------------ a pool of pages
+
+    def extend(self, weights: dict, ids: torch.Tensor, batch, *, want_logits: bool = True) -> dict:
+        """New tokens of many sequences over a pool of cache pages (`paged.PagePool`, `paged.PagedBatch`): prompts, chunks of prompts, known turns and single tokens
+        side by side.  ids: int64 [batch.tokens] on the device, sequence after sequence; batch.kv_len counts them already.  Writes their K and V rows into the pages and
+        returns `logits` [B, vocab] (None without want_logits) and `next_token` [B] of every sequence's last new token, fresh tensors.  Enqueues on the current stream
+        without synchronising; `status()` reports descriptors that do not fit.
+
+        The engine needs max_batch >= B and max_tokens (or max_batch) of at least the tokens of a call and 4.  Activations are rounded to bf16 as a prompt's are
+        (`bind_sequences` keeps a decode step's closer to fp32, over contiguous caches)."""
+        pool = batch.pool
+        if pool.layers != self.layers or pool.device != self.device:
+            raise ValueError(f"extend: the pool holds {pool.layers} layers on {pool.device}, the engine {self.layers} on {self.device}")
+        if ids.dtype != torch.int64 or ids.shape != (batch.tokens,) or ids.device != self.device or not ids.is_contiguous():
+            raise ValueError(f"extend: ids: expected a contiguous int64 [{batch.tokens}] on {self.device}, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
+        self._set_weights(weights)
+        logits = torch.empty((batch.batch, self.vocab), dtype=torch.float32, device=self.device) if want_logits else None
+        nxt = torch.empty(batch.batch, dtype=torch.int64, device=self.device)
+        space = torch.empty(batch.workspace_bytes(Q_HEADS), dtype=torch.uint8, device=self.device)
+        a = _cabi.ExtendArgs(ctypes.pointer(batch.view(0)), pool.k.stride(0), ids.data_ptr(), logits.data_ptr() if want_logits else None, nxt.data_ptr(), space.data_ptr(), space.numel())
+        _cabi.check(self.lib, self.handle, self.lib.q3_extend(self.handle, ctypes.byref(a), torch.cuda.current_stream(self.device).cuda_stream), "q3_extend")
+        return {"logits": logits, "next_token": nxt}
 
     # ------------------------------------------------------------------ bound path
 

@@ -100,7 +100,8 @@ class PagedBatch:
 
     def workspace_bytes(self, q_heads: int) -> int:
         if self._space is None:
-            n = self.lib.q3_paged_attn_workspace(ctypes.byref(self.view(0)), q_heads)
+            with _on(self.pool.device):
+                n = self.lib.q3_paged_attn_workspace(ctypes.byref(self.view(0)), q_heads)
             if n < 0:
                 _cabi.check(self.lib, None, int(n), "q3_paged_attn_workspace")
             self._space = n
