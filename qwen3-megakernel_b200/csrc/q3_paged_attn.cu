@@ -21,15 +21,19 @@ namespace q3 {
 struct PagedAttnArgs {
     PagedView c;
     PgShape sh;
-    int group;                       // q heads a kv head serves
+    int group_log;                   // a kv head serves 2^group_log q heads
     const unsigned char* q;
     unsigned char* out;
     long long q_token, q_head, o_token, o_head;      // bytes
     float scale;                     // times log2(e): scores are kept in units of log2
+    struct PgCut* cuts;              // one a block
     float* part;                     // two partial results a block
     int least;                       // units a block takes at least
     uint32_t* status;
 };
+
+// What a block leaves behind: the item that is cut at its end and began in its run, to be put together of the results of `parts` blocks (0: none)
+struct PgCut { int parts, slot, b, h, r, unused[3]; };
 
 __device__ __forceinline__ float pg_ex2(float x) {
     float y;
@@ -65,22 +69,27 @@ struct PgFp16 {
 };
 
 // What a segment is about: the keys [key0, key1) that its unit range holds, and per row of the tile (token row / group, q head row % group of the kv head's)
+__device__ __forceinline__ void pg_leave_cut(const PagedAttnArgs& a, const PgWalk& w, bool first, long long total, int blocks) {      // one thread, for a run's last segment
+    const PgSegment& s = w.s;
+    const bool begins = !w.whole() && s.k0 == 0;
+    a.cuts[blockIdx.x] = PgCut{begins ? pg_runs_before(total, blocks, w.at + s.units) - (int)blockIdx.x : 0, first ? 0 : 1, s.b, s.h, s.r, {0, 0, 0}};
+}
 struct PgKeys { int key0, key1, qpos0, rows; };
 __device__ __forceinline__ PgKeys pg_keys(const PagedAttnArgs& a, const PgSegment& s) {
     PgKeys k;
-    const int tok0 = s.r * a.sh.tile, live = min(a.sh.tile, s.seq.q - tok0);
+    const int tok0 = s.r << a.sh.tile_log, live = min(1 << a.sh.tile_log, s.seq.q - tok0);
     k.qpos0 = s.seq.kv - s.seq.q + tok0;                       // position of the tile's first token (below 0: a token without a position)
     const int seen = max(0, min(s.seq.kv, k.qpos0 + live));
-    k.key0 = min(s.k0 * a.sh.unit, seen);
-    k.key1 = min((long long)s.k1 * a.sh.unit, (long long)seen);
-    k.rows = live * a.group;
+    k.key0 = (int)min((long long)s.k0 << a.sh.unit_log, (long long)seen);
+    k.key1 = (int)min((long long)s.k1 << a.sh.unit_log, (long long)seen);
+    k.rows = live << a.group_log;
     return k;
 }
 __device__ __forceinline__ const unsigned char* pg_q_row(const PagedAttnArgs& a, const PgSegment& s, int row) {
-    return a.q + (long long)(s.seq.q0 + s.r * a.sh.tile + row / a.group) * a.q_token + (long long)(s.h * a.group + row % a.group) * a.q_head;
+    return a.q + (long long)(s.seq.q0 + (s.r << a.sh.tile_log) + (row >> a.group_log)) * a.q_token + (long long)((s.h << a.group_log) + (row & ((1 << a.group_log) - 1))) * a.q_head;
 }
 __device__ __forceinline__ unsigned char* pg_o_row(const PagedAttnArgs& a, const PgSegment& s, int row) {
-    return a.out + (long long)(s.seq.q0 + s.r * a.sh.tile + row / a.group) * a.o_token + (long long)(s.h * a.group + row % a.group) * a.o_head;
+    return a.out + (long long)(s.seq.q0 + (s.r << a.sh.tile_log) + (row >> a.group_log)) * a.o_token + (long long)((s.h << a.group_log) + (row & ((1 << a.group_log) - 1))) * a.o_head;
 }
 
 // A row again, key by key, reading only what it sees: for rows whose result is not finite.  A product adds 0 * v for keys that a row does not see
@@ -92,7 +101,7 @@ __device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment
     auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "n"(WARPS * 32) : "memory"); };
     const uint2 q2 = *reinterpret_cast<const uint2*>(pg_q_row(a, s, row) + lane * 8);
     const float2 qa = T::unpack(q2.x), qb = T::unpack(q2.y);
-    const int end = min(k.key1, k.qpos0 + row / a.group + 1);
+    const int end = min(k.key1, k.qpos0 + (row >> a.group_log) + 1);
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int p = k.key0 + warp; p < end; p += WARPS) {
         const int page = pg_page(a.c, s.b, p);
@@ -144,7 +153,7 @@ __device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment
 // fragment of them serves all NB blocks.
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int PR_WARPS = 4, PR_THREADS = PR_WARPS * 32, PR_TILE = 16, PR_STAGES = 3, PR_HALF = PR_TILE * 256, PR_STAGE = 2 * PR_HALF;
-constexpr int PR_UNIT = 64;                           // keys of a unit: a tile of 16 for every warp
+constexpr int PR_UNIT_LOG = 6;                        // 64 keys a unit: a tile of 16 for every warp
 constexpr size_t PR_SMEM = (size_t)PR_WARPS * PR_STAGES * PR_STAGE;
 constexpr int PG_PART = 132;                          // floats of a row of a partial result: maximum, sum, two unused, output
 
@@ -172,9 +181,11 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
     pg_block_prefix<PR_THREADS>(a.sh, a.c.q_start, a.c.kv_len, s_prefix, s_sum);
     const long long total = s_prefix[a.sh.batch];
     const int blocks = pg_blocks(total, (int)gridDim.x, a.least);
-    if ((int)blockIdx.x >= blocks) return;
     PgWalk walk;
-    if (!walk.begin(a.sh, s_prefix, a.c.q_start, a.c.kv_len, pg_run_start(total, blocks, blockIdx.x), pg_run_start(total, blocks, blockIdx.x + 1))) return;
+    if ((int)blockIdx.x >= blocks || !walk.begin(a.sh, s_prefix, a.c.q_start, a.c.kv_len, pg_run_start(total, blocks, blockIdx.x), pg_run_start(total, blocks, blockIdx.x + 1))) {
+        if (tid == 0) a.cuts[blockIdx.x].parts = 0;
+        return;
+    }
     unsigned char* const stage0 = pr_raw + (size_t)warp * PR_STAGES * PR_STAGE;
     float* const s_o = reinterpret_cast<float*>(stage0);
     const int page_mask = (1 << a.c.page_log) - 1;
@@ -266,7 +277,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
                 for (int e = 0; e < 2; ++e) {
                     float sa = c[nb][e] * a.scale, sb = c[nb][2 + e] * a.scale;
                     if (!all) {
-                        const int last = there ? min(w1 - 1, k.qpos0 + (8 * nb + 2 * ft + e) / a.group) : -1;
+                        const int last = there ? min(w1 - 1, k.qpos0 + ((8 * nb + 2 * ft + e) >> a.group_log)) : -1;
                         if (pa > last) sa = -INFINITY;
                         if (pa + 8 > last) sb = -INFINITY;
                     }
@@ -363,7 +374,10 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
             store(row, s_res[0], s_res[1], s_res[4 + tid]);
         }
         __syncthreads();
-        if (tid == 0) s_bad = 0;
+        if (tid == 0) {
+            s_bad = 0;
+            if (walk.at + s.k1 - s.k0 >= walk.end) pg_leave_cut(a, walk, first, total, blocks);
+        }
         first = false;
     } while (walk.next(a.sh, a.c.q_start, a.c.kv_len));
 }
@@ -420,6 +434,31 @@ __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t* r) {
                  ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
 }
+__device__ __forceinline__ float pt_max3(float a, uint32_t b, uint32_t c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return d;
+}
+__device__ __forceinline__ uint64_t pt_pair(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 pt_unpair(uint64_t v) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+    return d;
+}
+__device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ void pt_init(uint64_t* bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(bar)), "r"(count) : "memory"); }
 __device__ __forceinline__ void pt_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(bar)), "r"(bytes) : "memory");
@@ -449,7 +488,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     pg_block_prefix<PT_THREADS>(a.sh, a.c.q_start, a.c.kv_len, s_prefix, s_sum);
     const long long total = s_prefix[a.sh.batch];
     const int blocks = pg_blocks(total, (int)gridDim.x, a.least);
-    if ((int)blockIdx.x >= blocks) return;
+    if ((int)blockIdx.x >= blocks) {
+        if (tid == 0) a.cuts[blockIdx.x].parts = 0;
+        return;
+    }
     unsigned char* const sKV = pt_raw + 2 * PT_TILE;  // stage s: K at s * 2 * PT_TILE, V right behind it
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -500,7 +542,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
                     for (int b = 0; b < 2; ++b)       // rows past q are zeros
                         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                     ::"r"(tc_smem(pt_raw + buf * PT_TILE + b * PT_BOX)), "l"(&tm_q), "r"(64 * b), "r"(w.s.h * a.group), "r"(w.s.seq.q0 + w.s.r * a.sh.tile),
+                                     ::"r"(tc_smem(pt_raw + buf * PT_TILE + b * PT_BOX)), "l"(&tm_q), "r"(64 * b), "r"(w.s.h << a.group_log), "r"(w.s.seq.q0 + (w.s.r << a.sh.tile_log)),
                                        "r"(tc_smem(&q_full[buf])) : "memory");
                 }
                 armed_q = ++n_q;
@@ -611,21 +653,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         while (left) {
             const PgKeys k = pg_keys(a, w.s);
             const int n = pt_tiles(k);
-            const int last = min(k.qpos0 + row / a.group, k.key1 - 1);       // the last key this row sees
+            const int last = min(k.qpos0 + (row >> a.group_log), k.key1 - 1);       // the last key this row sees
             const bool live = quad * 32 < k.rows;                            // (the warp has a row)
             const int t0 = (grp ^ g0) & 1;
             float m = -INFINITY, lsum = 0.f;
-            auto pages_of = [&](int t) {             // bit i: whether keys 16 i .. of tile t have a page (or nobody sees them)
-                const int key = k.key0 + t * PT_KEYS + 16 * (lane & 7);
-                const bool there = t >= n || key >= k.key1 || pg_page(a.c, w.s.b, key) >= 0;
-                return there;
+            // whether all pages of the segment are there (usually), and which of a tile's are: bit i for the keys 16 i ..
+            bool every = true;
+            for (int i = (k.key0 >> a.c.page_log) + lane; n > 0 && i <= (k.key1 - 1) >> a.c.page_log; i += 32) every = every && (unsigned)a.c.table[(long long)w.s.b * a.c.table_stride + i] < (unsigned)a.c.n_pages;
+            every = __all_sync(0xffffffffu, every);
+            auto pages_of = [&](int tile0) {
+                const int key = tile0 + 16 * (lane & 7);
+                return __ballot_sync(0xffffffffu, key >= k.key1 || pg_page(a.c, w.s.b, key) >= 0) & 0xffu;
             };
-            bool there = pages_of(t0);
             for (int t = t0; t < n; t += 2) {
                 const int g = g0 + t, tile0 = k.key0 + t * PT_KEYS;
                 const uint32_t turn = (uint32_t)(g >> 1) & 1u;
-                const unsigned pages = __ballot_sync(0xffffffffu, there) & 0xffu;
-                there = pages_of(t + 2);
+                const unsigned pages = every ? 0xffu : pages_of(tile0);
                 pt_wait_warp(&s_full[grp], turn, &abort_flag, a.status, 88);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (live) {
@@ -644,7 +687,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     }
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) { x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[0][j])); x[2 + (j & 1)] = fmaxf(x[2 + (j & 1)], __uint_as_float(r[1][j])); }
+                    for (int j = 0; j < 32; j += 4) {
+                        x[0] = pt_max3(x[0], r[0][j], r[0][j + 1]); x[1] = pt_max3(x[1], r[0][j + 2], r[0][j + 3]);
+                        x[2] = pt_max3(x[2], r[1][j], r[1][j + 1]); x[3] = pt_max3(x[3], r[1][j + 2], r[1][j + 3]);
+                    }
                     const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                     // the row's other half is a thread of the warp four further; behind the barrier both have read their part of S, too
                     s_max[grp][turn][part][row] = x0;
@@ -670,19 +716,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                         }
                     }
                     const float ms = m == -INFINITY ? 0.f : m;               // (nothing seen so far: every exponential is 0)
-                    float psum0 = 0.f, psum1 = 0.f;
+                    const uint64_t c2 = pt_pair(a.scale, a.scale), m2 = pt_pair(-ms, -ms);
+                    uint64_t sum2[2] = {0ull, 0ull};                         // (two elements an instruction where it is one of the FMA pipe's)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float e0 = pg_ex2(fmaf(__uint_as_float(r[h][2 * j]), a.scale, -ms)), e1 = pg_ex2(fmaf(__uint_as_float(r[h][2 * j + 1]), a.scale, -ms));
-                            psum0 += e0; psum1 += e1;
+                            const float2 x2 = pt_unpair(pt_fma2(pt_pair(__uint_as_float(r[h][2 * j]), __uint_as_float(r[h][2 * j + 1])), c2, m2));
+                            const float e0 = pg_ex2(x2.x), e1 = pg_ex2(x2.y);
+                            sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(e0, e1));
                             pk[j] = T::pack(e0, e1);
                         }
                         pt_st16(ts + (uint32_t)(part * 32 + h * 16), pk);
                     }
-                    lsum += psum0 + psum1;
+                    const float2 s2 = pt_unpair(pt_add2(sum2[0], sum2[1]));
+                    lsum += s2.x + s2.y;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 if (tile0 + PT_KEYS > k.key1) {
@@ -794,6 +843,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 ++n_q;
             }
             g0 += n;
+            if (tid == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
             first = false;
             left = w.next(a.sh, qs, kl);
         }
@@ -818,32 +868,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Items that were cut: a block per cut, the one at an item's first cut puts the item together.  A warp a row, a lane four dims.
+// Items that were cut: the block in whose run an item began has left word of it.  A warp a row, a lane four dims; the parts are added in the order of their keys.
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int PJ_THREADS = 128;
 
 template <typename T>
-__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnArgs a, int grid, int part_rows) {
-    __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PJ_THREADS / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnArgs a, int part_rows) {
     pdl_launch();
     pdl_wait();
-    pg_block_prefix<PJ_THREADS>(a.sh, a.c.q_start, a.c.kv_len, s_prefix, s_sum);
-    const long long total = s_prefix[a.sh.batch];
-    const int blocks = pg_blocks(total, grid, a.least), cut = (int)blockIdx.x + 1;
-    if (cut >= blocks) return;
-    const long long at = pg_run_start(total, blocks, cut);
-    PgWalk walk;
-    if (!walk.begin(a.sh, s_prefix, a.c.q_start, a.c.kv_len, at, at + 1)) return;
-    const PgSegment& s = walk.s;
-    const long long from = at - s.k0, to = from + s.units, before = pg_run_start(total, blocks, cut - 1);
-    if (s.k0 == 0 || before > from) return;            // no item is cut here, or this is not its first cut
-    const int live = min(a.sh.tile, s.seq.q - s.r * a.sh.tile) * a.group;
-    int parts = 1;
-    while (cut + parts - 1 < blocks && pg_run_start(total, blocks, cut + parts - 1) < to) ++parts;      // blocks cut - 1 .. cut + parts - 2
-    const size_t slot0 = (size_t)2 * (cut - 1) + (before == from ? 0 : 1);
-    auto part = [&](int i, int row) { return a.part + ((i == 0 ? slot0 : (size_t)2 * (cut - 1 + i)) * part_rows + row) * PG_PART; };
-    for (int row = blockIdx.y * (PJ_THREADS / 32) + warp; row < live; row += gridDim.y * (PJ_THREADS / 32)) {
+    const int lane = threadIdx.x & 31, block = blockIdx.x;
+    const int4 cut = *reinterpret_cast<const int4*>(&a.cuts[block]);
+    const int parts = cut.x;
+    if (parts == 0) return;
+    PgSegment s;
+    s.b = cut.z; s.h = cut.w; s.r = a.cuts[block].r;
+    s.seq = pg_seq(a.sh, a.c.q_start, a.c.kv_len, s.b);
+    const int live = min(1 << a.sh.tile_log, s.seq.q - (s.r << a.sh.tile_log)) << a.group_log;
+    auto part = [&](int i, int row) { return a.part + ((size_t)(2 * (block + i) + (i == 0 ? cut.y : 0)) * part_rows + row) * PG_PART; };
+    for (int row = blockIdx.y * (PJ_THREADS / 32) + (threadIdx.x >> 5); row < live; row += gridDim.y * (PJ_THREADS / 32)) {
         float M = -INFINITY;
         bool nan = false;
         for (int i = lane; i < parts; i += 32) { const float x = part(i, row)[0]; M = fmaxf(M, x); nan = nan || x != x; }
@@ -859,13 +901,18 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
                 w = ml.x == -INFINITY ? 0.f : ml.x == Ms ? 1.f : pg_ex2(ml.x - Ms);
                 lw = ml.x == -INFINITY ? 0.f : ml.y * w;
             }
+            L += warp_sum(lw);
             const int n = min(32, parts - i0);
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                L += __shfl_sync(0xffffffffu, lw, i);
-                const float4 x = *reinterpret_cast<const float4*>(part(i0 + i, row) + 4 + lane * 4);
-                if (wi != 0.f) { v.x = fmaf(x.x, wi, v.x); v.y = fmaf(x.y, wi, v.y); v.z = fmaf(x.z, wi, v.z); v.w = fmaf(x.w, wi, v.w); }
+            for (int i1 = 0; i1 < n; i1 += 8) {       // eight parts' loads under way
+                float4 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i1 + i < n) x[i] = *reinterpret_cast<const float4*>(part(i0 + i1 + i, row) + 4 + lane * 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float wi = __shfl_sync(0xffffffffu, w, (i1 + i) & 31);
+                    if (i1 + i < n && wi != 0.f) { v.x = fmaf(x[i].x, wi, v.x); v.y = fmaf(x[i].y, wi, v.y); v.z = fmaf(x[i].z, wi, v.z); v.w = fmaf(x[i].w, wi, v.w); }
+                }
             }
         }
         const float r = L > 0.f || L != L ? 1.f / L : 0.f;
@@ -876,16 +923,35 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
 // ------------------------------------------------------------------------------------------------------------------------------
 // New tokens of a sequence up to which the products are the few-row kernel's: 32 rows with all q heads of a kv head.
 static bool pg_few(int max_new, int group) { return max_new * (long long)group <= 32; }
+static int pg_log(int n) {
+    int l = 0;
+    while ((1 << l) < n) ++l;
+    return l;
+}
+
+// what a kernel asks for beyond the defaults, once for every device (a benign race between host threads: the same value is set)
+template <typename K>
+static cudaError_t pg_shared(K* kernel, size_t bytes, bool (&set)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!set[dev]) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)) != cudaSuccess) return e;
+        set[dev] = true;
+    }
+    return cudaSuccess;
+}
 
 template <typename T, int NB>
 static cudaError_t launch_rows(PagedAttnArgs& a, cudaStream_t st) {
-    a.sh.unit = PR_UNIT;
-    a.sh.tile = 8 * NB / a.group;
+    a.sh.unit_log = PR_UNIT_LOG;
+    a.sh.tile_log = (NB == 1 ? 3 : NB == 2 ? 4 : 5) - a.group_log;
     a.least = 1;
     const int grid = 2 * tc_sm_count();
-    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PR_SMEM);
+    static bool set[64] = {};
+    cudaError_t e = pg_shared(paged_rows_kernel<T, NB>, PR_SMEM, set);
     if (e == cudaSuccess) e = launch_chain(paged_rows_kernel<T, NB>, dim3(grid), dim3(PR_THREADS), PR_SMEM, st, a);
-    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid - 1, 2 * NB), dim3(PJ_THREADS), 0, st, a, grid, 8 * NB);
+    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid, 2 * NB), dim3(PJ_THREADS), 0, st, a, 8 * NB);
     return e;
 }
 
@@ -909,25 +975,26 @@ static bool pg_make_map(CUtensorMap* m, bool bf, const void* p, int rank, const 
 
 template <typename T>
 static cudaError_t launch_tiles(PagedAttnArgs& a, int q_heads, cudaStream_t st) {
-    a.sh.unit = PT_KEYS;
-    a.sh.tile = 128 / a.group;
+    a.sh.unit_log = 7;
+    a.sh.tile_log = 7 - a.group_log;
     a.least = 1;
     CUtensorMap q, k, v;
     const uint64_t dq[3] = {HEAD_DIM, (uint64_t)q_heads, (uint64_t)a.sh.n_tokens}, dk[4] = {HEAD_DIM, 1ull << a.c.page_log, (uint64_t)a.sh.heads, (uint64_t)a.c.n_pages};
     const int64_t sq[2] = {a.q_head, a.q_token}, sk[3] = {a.c.slot_bytes, a.c.head_bytes, a.c.page_bytes};
-    const uint32_t bq[3] = {64, (uint32_t)a.group, (uint32_t)a.sh.tile}, bk[4] = {64, 1u << (a.c.page_log < 7 ? a.c.page_log : 7), 1, 1};
+    const uint32_t bq[3] = {64, 1u << a.group_log, 1u << a.sh.tile_log}, bk[4] = {64, 1u << (a.c.page_log < 7 ? a.c.page_log : 7), 1, 1};
     if (!pg_make_map(&q, T::BF, a.q, 3, dq, sq, bq) || !pg_make_map(&k, T::BF, a.c.k, 4, dk, sk, bk) || !pg_make_map(&v, T::BF, a.c.v, 4, dk, sk, bk)) return cudaErrorInvalidValue;
     const int grid = tc_sm_count();
-    cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PT_SMEM);
+    static bool set[64] = {};
+    cudaError_t e = pg_shared(paged_tile_kernel<T>, PT_SMEM, set);
     if (e == cudaSuccess) e = launch_chain(paged_tile_kernel<T>, dim3(grid), dim3(PT_THREADS), PT_SMEM, st, q, k, v, a);
-    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid - 1, 8), dim3(PJ_THREADS), 0, st, a, grid, 128);
+    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid, 16), dim3(PJ_THREADS), 0, st, a, 128);
     return e;
 }
 
 template <typename T>
 static cudaError_t launch_attn(PagedAttnArgs& a, int max_new, int q_heads, cudaStream_t st) {
-    if (!pg_few(max_new, a.group)) return launch_tiles<T>(a, q_heads, st);
-    const int cols = max_new * a.group;
+    if (!pg_few(max_new, 1 << a.group_log)) return launch_tiles<T>(a, q_heads, st);
+    const int cols = max_new << a.group_log;
     return cols <= 8 ? launch_rows<T, 1>(a, st) : cols <= 16 ? launch_rows<T, 2>(a, st) : launch_rows<T, 4>(a, st);
 }
 
@@ -968,13 +1035,14 @@ PagedView paged_view(const q3_paged* c) {
 
 using namespace q3;
 
-// two partial results a block: 32 rows at most for each of two blocks an SM, or 128 for one
+static int64_t pg_cut_bytes() { return ((int64_t)2 * tc_sm_count() * (int64_t)sizeof(PgCut) + 1023) / 1024 * 1024; }
+// a record a block, two partial results a block: 32 rows at most for each of two blocks an SM, or 128 for one
 extern "C" int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads) {
     if (!c || q_heads < 1) return engine_fail(nullptr, Q3_ERR_INVALID, "q3_paged_attn_workspace: bad argument");
     const int sms = tc_sm_count();
     if (sms < 1) return engine_fail(nullptr, Q3_ERR_CUDA, "q3_paged_attn_workspace: no CUDA device");
     const int group = q_heads / (c->kv_heads < 1 ? 1 : c->kv_heads);
-    return (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 32 : 128) * PG_PART * 4;
+    return pg_cut_bytes() + (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 32 : 128) * PG_PART * 4;
 }
 
 extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, void* stream) {
@@ -999,12 +1067,13 @@ extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, voi
     PagedAttnArgs a{};
     a.c = paged_view(c);
     a.sh.heads = c->kv_heads; a.sh.batch = c->batch; a.sh.n_tokens = c->n_tokens; a.sh.most_keys = c->table_pages * c->page_size;
-    a.group = group;
+    a.group_log = pg_log(group);
     a.q = static_cast<const unsigned char*>(p->q);
     a.out = static_cast<unsigned char*>(p->out);
     a.q_token = 2 * p->q_token; a.q_head = 2 * p->q_head; a.o_token = 2 * p->out_token; a.o_head = 2 * p->out_head;
     a.scale = p->scale * 1.4426950408889634f;
-    a.part = static_cast<float*>(p->workspace);
+    a.cuts = static_cast<PgCut*>(p->workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + pg_cut_bytes());
     a.status = p->status;
     cudaStream_t st = (cudaStream_t)stream;
     const int max_new = c->max_new < 1 ? 1 : c->max_new;

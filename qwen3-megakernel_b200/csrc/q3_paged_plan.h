@@ -18,8 +18,8 @@ namespace q3 {
 constexpr int PG_MAX_BATCH = 1024;    // sequences of a call: their prefix sums lie in shared memory
 
 struct PgShape {
-    int tile;         // new tokens of a tile, a power of two, at most `unit`
-    int unit;         // keys of a unit, a power of two
+    int tile_log;     // a tile is 2^tile_log new tokens,
+    int unit_log;     // a unit 2^unit_log keys, at least as many
     int heads;        // kv heads
     int batch;
     int n_tokens;     // rows of q: nothing behind them is read or written
@@ -38,25 +38,26 @@ PG_HD PgSeq pg_seq(const PgShape& s, const int* q_start, const int* kv_len, int 
     return r;
 }
 
-PG_HD int pg_tiles(const PgShape& s, const PgSeq& q) { return (int)(((long long)q.q + s.tile - 1) / s.tile); }
+PG_HD int pg_tiles(const PgShape& s, const PgSeq& q) { return (int)(((long long)q.q + (1 << s.tile_log) - 1) >> s.tile_log); }
 
 // Tile r sees the keys before position kv - q + min((r + 1) tile, q).  (Fewer keys than new tokens: counted as if the chunk began at position 0, so that
 // an item has one unit at least; what its tokens see is looked up by position.)
 PG_HD long long pg_tile_units(const PgShape& s, const PgSeq& q, int r) {
-    const long long c0 = q.kv > q.q ? q.kv - q.q : 0, last = (long long)(r + 1) * s.tile < q.q ? (long long)(r + 1) * s.tile : q.q;
-    return (c0 + last + s.unit - 1) / s.unit;
+    const long long c0 = q.kv > q.q ? q.kv - q.q : 0, full = (long long)(r + 1) << s.tile_log, last = full < q.q ? full : q.q;
+    return (c0 + last + (1 << s.unit_log) - 1) >> s.unit_log;
 }
 
-// sum of floor(i / n) over i = 0 .. y
-PG_HD long long pg_floor_sum(long long y, long long n) {
-    const long long q = (y + 1) / n, rem = (y + 1) % n;
-    return n * (q * (q - 1) / 2) + q * rem;
+// sum of floor(i / 2^n) over i = 0 .. y
+PG_HD long long pg_floor_sum(long long y, int n) {
+    const long long q = (y + 1) >> n, rem = (y + 1) & ((1ll << n) - 1);
+    return ((q * (q - 1) / 2) << n) + q * rem;
 }
 
-// Units of the tiles 0 .. x - 1, all of them but possibly the last tile of the sequence full: with n = unit / tile and c0 + tile + unit - 1 = tile * a + rest,
-// tile r has floor((a + r) / n) units.
+// Units of the tiles 0 .. x - 1, all of them but possibly the last tile of the sequence full: with c0 + tile + unit - 1 = tile * a + rest,
+// tile r has floor((a + r) / (unit / tile)) units.
 PG_HD long long pg_units_before(const PgShape& s, const PgSeq& q, int x) {
-    const long long c0 = q.kv > q.q ? q.kv - q.q : 0, n = s.unit / s.tile, a = (c0 + s.tile + s.unit - 1) / s.tile;
+    const long long c0 = q.kv > q.q ? q.kv - q.q : 0, a = (c0 + (1 << s.tile_log) + (1 << s.unit_log) - 1) >> s.tile_log;
+    const int n = s.unit_log - s.tile_log;
     return pg_floor_sum(a + x - 1, n) - pg_floor_sum(a - 1, n);
 }
 
@@ -72,6 +73,8 @@ PG_HD int pg_blocks(long long total, int blocks, int least) {
     return (int)(n < blocks ? n : blocks);
 }
 PG_HD long long pg_run_start(long long total, int blocks, int i) { return total * i / blocks; }     // (total < 2^53: 2^31 keys a sequence, 2^10 sequences, 2^10 blocks)
+// how many blocks begin before unit x: the one that holds unit x - 1 and all before it
+PG_HD int pg_runs_before(long long total, int blocks, long long x) { return (int)((x * blocks + total - 1) / total); }
 
 struct PgSegment {
     PgSeq seq;

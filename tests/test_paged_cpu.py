@@ -22,7 +22,7 @@ int main() {
     for (int it = 0; it < 20000; ++it) {
         PgShape s;
         const int log = 6 + rand() % 2;
-        s.unit = 1 << log; s.tile = 1 << (rand() % (log + 1)); s.heads = 1 + rand() % 8; s.batch = 1 + rand() % 6;
+        s.unit_log = log; s.tile_log = rand() % (log + 1); s.heads = 1 + rand() % 8; s.batch = 1 + rand() % 6;
         std::vector<int> qs(s.batch + 1), kv(s.batch);
         qs[0] = rand() % 4 ? 0 : rand() % 9;
         for (int b = 0; b < s.batch; ++b) {
@@ -44,7 +44,7 @@ int main() {
             long long u = 0;
             for (int r = 0; r < pg_tiles(s, q); ++r) {
                 if (pg_units_before(s, q, r) != u) return fail("units before a tile");
-                if (pg_tile_units(s, q, r) * s.unit < q.kv - q.q + (r + 1 < pg_tiles(s, q) ? (r + 1) * s.tile : q.q)) return fail("a tile sees keys that no unit holds");
+                if ((pg_tile_units(s, q, r) << s.unit_log) < q.kv - q.q + (r + 1 < pg_tiles(s, q) ? (r + 1) << s.tile_log : q.q)) return fail("a tile sees keys that no unit holds");
                 u += pg_tile_units(s, q, r);
             }
             if (u != pg_head_units(s, q)) return fail("units of a head");
@@ -71,6 +71,9 @@ int main() {
                 k = x.k1;
                 if (k == g.units) { k = 0; ++at; }
                 if (!w.whole()) ++cut;
+                int runs = 0;
+                while (runs < n && pg_run_start(total, n, runs) < w.at + x.units - x.k0) ++runs;
+                if (pg_runs_before(total, n, w.at + x.units - x.k0) != runs) return fail("runs before the end of an item");
                 ++segment;
             } while (w.next(s, qs.data(), kv.data()));
             if (cut > 2 || !segment) return fail("a run holds more than two parts of items, or nothing");
