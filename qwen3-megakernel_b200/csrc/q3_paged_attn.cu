@@ -385,17 +385,17 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
 // ------------------------------------------------------------------------------------------------------------------------------
 // Chunks of new tokens: 128 rows (128 / group tokens of every q head of a kv head) against tiles of 128 keys on tcgen05.mma, accumulators in TMEM.
 //     S  = Q K^T     M 128 x N 128 keys x K 128 dims, both K-major        -> TMEM columns [0, 128) / [128, 256), by the parity of the tile
-//     P  = 2^(S - m) two groups of eight warps, two threads a row (64 keys each); group g takes the tiles of parity g, so that one group's exponentials
+//     P  = 2^(S - m) two groups of four warps, a thread a row; group g takes the tiles of parity g, so that one group's exponentials
 //                    run while the tensor pipe and the hand-offs of the other's tile do.  P takes the place of S in TMEM
 //     O += P V       V is the MN-major operand straight from its tile; an O a group -> columns [256, 384) / [384, 512)
-// as in q3_prefill_attn_tc.cu, and beyond it: K and V come page by page (a TMA box a page and half of the dims; a page that is not there, or that no row of the tile sees, lies
-// outside the tensor and reads as zeros), and a block walks the segments of its run without draining: tiles are counted over all of them, the next segment's Q
-// has a buffer of its own, its first scores are under way while the last one's rows are finished.
+// K and V come page by page (a TMA box a page and half of the dims; a page that is not there, or that no row of the tile sees, lies
+// outside the tensor and reads as zeros), each by a warp of its own, and a block walks the segments of its run without draining: tiles are counted over all of them, the next
+// segment's Q has a buffer of its own, its first scores are under way while the last one's rows are finished.
 // O is rescaled only when a score exceeds the maximum that P is taken under by 2^8.
 // A wait that gives up lets every later one give up at once; all warps still meet at every barrier, rows that are not finished become NaN, and the block drains
 // what is under way before it leaves.
 // ------------------------------------------------------------------------------------------------------------------------------
-constexpr int PT_SOFT = 512, PT_THREADS = PT_SOFT + 64;       // warps 0..15 softmax and output, 16 TMA, 17 MMA and TMEM
+constexpr int PT_SOFT = 256, PT_WARPS = PT_SOFT / 32, PT_THREADS = PT_SOFT + 96;      // warps 0..7 softmax and output, 8 TMA of Q and K, 9 TMA of V, 10 MMA and TMEM
 constexpr int PT_KEYS = 128;                                  // keys of a tile, the unit of work
 constexpr uint32_t PT_BOX = 128 * 128, PT_TILE = 2 * PT_BOX;  // [128 rows][64 dims] with 128-byte swizzle; 128 x 128
 constexpr size_t PT_SMEM = 2 * PT_TILE + 2 * 2 * PT_TILE;     // two of Q, two stages of K and V
@@ -477,8 +477,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free, drain_bar;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_flag;
-    __shared__ float s_max[2][2][2][128];           // per group and parity of its tiles: the tile's maximum of a row's two halves
-    __shared__ float s_m[2][128], s_l[2][2][128];   // at a segment's end: per group, a row's maximum and the two halves of its sum
+    __shared__ float s_m[2][128], s_l[2][128];      // at a segment's end: per group, a row's maximum and sum
     __shared__ unsigned s_bad[4];
     __shared__ float s_res[132];
 
@@ -496,16 +495,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
             pt_init(&k_full[s], 1); pt_init(&v_full[s], 1); pt_init(&k_empty[s], 1); pt_init(&v_empty[s], 1);
-            pt_init(&q_full[s], 1); pt_init(&q_empty[s], PT_SOFT / 32);
-            pt_init(&s_full[s], 1); pt_init(&p_full[s], 8); pt_init(&o_full[s], 1);
+            pt_init(&q_full[s], 1); pt_init(&q_empty[s], PT_WARPS);
+            pt_init(&s_full[s], 1); pt_init(&p_full[s], 4); pt_init(&o_full[s], 1);
         }
-        pt_init(&o_free, PT_SOFT / 32);
+        pt_init(&o_free, PT_WARPS);
         pt_init(&drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
         s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
     }
-    if (warp == PT_SOFT / 32 + 1) {
+    if (warp == PT_WARPS + 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base_s)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -516,25 +515,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const int *qs = a.c.q_start, *kl = a.c.kv_len;
     const long long from = pg_run_start(total, blocks, blockIdx.x), to = pg_run_start(total, blocks, blockIdx.x + 1);
 
-    int armed_k = 0, armed_v = 0, armed_q = 0;      // what the producer has requested
-    if (warp == PT_SOFT / 32) {
+    int armed = 0, armed_q = 0;                     // tiles of K (V) and of Q that this warp has requested
+    if (warp == PT_WARPS || warp == PT_WARPS + 1) {
         // ---------------------------------------------------------------------- TMA: a lane a box
+        const bool is_v = warp != PT_WARPS;
         const int rows_log = min(a.c.page_log, 7), boxes = PT_KEYS >> rows_log, j = lane >> 1, half = lane & 1;      // a page's rows are cut into boxes of 128 at most
         const bool mine = j < boxes;
+        const CUtensorMap* const map = is_v ? &tm_v : &tm_k;
+        uint64_t *const full = is_v ? v_full : k_full, *const empty = is_v ? v_empty : k_empty;
+        const uint32_t dst0 = tc_smem(sKV + (is_v ? PT_TILE : 0)) + (uint32_t)half * PT_BOX + ((uint32_t)j << (rows_log + 7));
         PgWalk w;
         bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
         int g = 0, n_q = 0;
         while (ok) {
             const PgKeys k = pg_keys(a, w.s);
-            const int n = pt_tiles(k);
-            auto page_of = [&](int t) {               // of this lane's box of tile t; n_pages: no such page, zeros
-                const int key = k.key0 + t * PT_KEYS + (j << rows_log);
-                if (!mine || key >= k.key1) return a.c.n_pages;
-                const int p = pg_page(a.c, w.s.b, key);
-                return p < 0 ? a.c.n_pages : p;
-            };
-            int page = n > 0 ? page_of(0) : 0;
-            if (n > 0) {
+            const int n = pt_tiles(k), key0 = k.key0 + (j << rows_log);
+            const int* const table = a.c.table + (long long)w.s.b * a.c.table_stride;
+            // the page of this lane's box of tile t, as the table has it
+            auto entry = [&](int t) { const int key = key0 + t * PT_KEYS; return mine && key < k.key1 ? table[key >> a.c.page_log] : -1; };
+            int next = n > 0 ? entry(0) : -1;
+            if (n > 0 && !is_v) {
                 const int buf = n_q & 1;
                 if (n_q >= 2 && !pt_wait_warp(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) break;
                 if (lane == 0) {
@@ -547,32 +547,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 }
                 armed_q = ++n_q;
             }
-            for (int t = 0; t < n && ok; ++t, ++g) {
-                const int s = g & 1, slot = (k.key0 + t * PT_KEYS + (j << rows_log)) & ((1 << a.c.page_log) - 1);
-                const uint32_t dst = tc_smem(sKV + (size_t)s * 2 * PT_TILE) + (uint32_t)half * PT_BOX + ((uint32_t)j << (rows_log + 7));
-                const int next = t + 1 < n ? page_of(t + 1) : 0;
-                // K and V of a tile share a stage but are released separately: K as soon as the tile's scores are there
-                ok = g < 2 || pt_wait_warp(&k_empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
+            for (int t = 0; t < n; ++t, ++g) {
+                const int s = g & 1, slot = (key0 + t * PT_KEYS) & ((1 << a.c.page_log) - 1);
+                const int page = (unsigned)next < (unsigned)a.c.n_pages ? next : a.c.n_pages;      // no such page: outside the tensor
+                if (t + 1 < n) next = entry(t + 1);  // (on its way while this tile is waited for)
+                ok = g < 2 || pt_wait_warp(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
                 if (!ok) break;
-                if (lane == 0) pt_expect(&k_full[s], PT_TILE);
+                if (lane == 0) pt_expect(&full[s], PT_TILE);
                 __syncwarp();
                 if (mine)
                     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                                 ::"r"(dst), "l"(&tm_k), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&k_full[s])) : "memory");
-                armed_k = g + 1;
-                ok = g < 2 || pt_wait_warp(&v_empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 82);
-                if (!ok) break;
-                if (lane == 0) pt_expect(&v_full[s], PT_TILE);
-                __syncwarp();
-                if (mine)
-                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                                 ::"r"(dst + PT_TILE), "l"(&tm_v), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&v_full[s])) : "memory");
-                armed_v = g + 1;
-                page = next;
+                                 ::"r"(dst0 + (uint32_t)s * 2u * PT_TILE), "l"(map), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&full[s])) : "memory");
+                armed = g + 1;
             }
             ok = ok && w.next(a.sh, qs, kl);
         }
-    } else if (warp == PT_SOFT / 32 + 1) {
+    } else if (warp == PT_WARPS + 2) {
         // ---------------------------------------------------------------------- MMA issuer
         if (elect_one()) {
             const uint32_t idesc_s = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), idesc_o = idesc_s | (1u << 16);
@@ -620,7 +610,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 for (int t = 0; t < n && ok; ++t, ++g) {
                     const int b = g & 1;
                     if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
-                    ok = ok && pt_wait(&p_full[b], (g >> 1) & 1, &abort_flag, a.status, 86) && pt_wait(&v_full[b], (g >> 1) & 1, &abort_flag, a.status, 87);
+                    ok = ok && pt_wait(&v_full[b], (g >> 1) & 1, &abort_flag, a.status, 87) && pt_wait(&p_full[b], (g >> 1) & 1, &abort_flag, a.status, 86);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t dvs = dv + (uint64_t)b * 2 * TILE;
@@ -643,10 +633,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
     } else {
         // ---------------------------------------------------------------------- softmax and output: row = TMEM lane
-        const int quad = warp & 3, row = quad * 32 + lane, grp = warp >> 3, part = (warp >> 2) & 1;   // part: 64 keys of a tile
+        const int quad = warp & 3, row = quad * 32 + lane, grp = warp >> 2;
         const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
-        const uint32_t ts = trow + (uint32_t)(grp * 128), to_o = trow + 256u + (uint32_t)(grp * 128 + part * 64);
-        auto meet = [&] { asm volatile("bar.sync 9, %0;" ::"n"(PT_SOFT) : "memory"); };
+        const uint32_t ts = trow + (uint32_t)(grp * 128), to_o = trow + 256u + (uint32_t)(grp * 128);
+        auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(PT_SOFT) : "memory"); };
         PgWalk w;
         bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
         int g0 = 0, n_q = 0;
@@ -672,30 +662,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 pt_wait_warp(&s_full[grp], turn, &abort_flag, a.status, 88);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (live) {
-                    uint32_t r[2][32];
-                    tc_ld32(r[0], ts + (uint32_t)(part * 64));
-                    tc_ld32(r[1], ts + (uint32_t)(part * 64 + 32));
+                    uint32_t r[4][32];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) tc_ld32(r[h], ts + (uint32_t)(h * 32));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (tile0 + PT_KEYS - 1 > k.qpos0 || tile0 + PT_KEYS > k.key1 || pages != 0xffu) {
-                        const int key = tile0 + part * 64;
-                        const unsigned gone = ~(pages >> (part * 4));
+                        const int most = last - tile0;
+                        const unsigned gone = ~pages;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (key + j > last || ((gone >> (j >> 4)) & 1u)) r[0][j] = 0xff800000u;            // -inf
-                            if (key + 32 + j > last || ((gone >> (2 + (j >> 4))) & 1u)) r[1][j] = 0xff800000u;
-                        }
+                        for (int h = 0; h < 4; ++h)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (h * 32 + j > most || ((gone >> (h * 2 + (j >> 4))) & 1u)) r[h][j] = 0xff800000u;            // -inf
                     }
                     float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        x[0] = pt_max3(x[0], r[0][j], r[0][j + 1]); x[1] = pt_max3(x[1], r[0][j + 2], r[0][j + 3]);
-                        x[2] = pt_max3(x[2], r[1][j], r[1][j + 1]); x[3] = pt_max3(x[3], r[1][j + 2], r[1][j + 3]);
-                    }
-                    const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                    // the row's other half is a thread of the warp four further; behind the barrier both have read their part of S, too
-                    s_max[grp][turn][part][row] = x0;
-                    asm volatile("bar.sync %0, 64;" ::"r"(1 + grp * 4 + quad) : "memory");
-                    const float top = fmaxf(x0, s_max[grp][turn][part ^ 1][row]) * a.scale;
+                    for (int j = 0; j < 32; j += 2)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) x[h] = pt_max3(x[h], r[h][j], r[h][j + 1]);
+                    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
                     const bool raise = !(top <= m + PT_LAG);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
@@ -705,7 +690,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                             pt_wait_warp(&o_full[grp], turn ^ 1u, &abort_flag, a.status, 89);
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                            for (int h = 0; h < 64; h += 16) {
+                            for (int h = 0; h < 128; h += 16) {
                                 uint32_t o[16];
                                 tc_ld16(o, to_o + (uint32_t)h);
                                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -719,7 +704,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     const uint64_t c2 = pt_pair(a.scale, a.scale), m2 = pt_pair(-ms, -ms);
                     uint64_t sum2[2] = {0ull, 0ull};                         // (two elements an instruction where it is one of the FMA pipe's)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < 4; ++h) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
@@ -728,7 +713,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                             sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(e0, e1));
                             pk[j] = T::pack(e0, e1);
                         }
-                        pt_st16(ts + (uint32_t)(part * 32 + h * 16), pk);
+                        pt_st16(ts + (uint32_t)(h * 16), pk);
                     }
                     const float2 s2 = pt_unpair(pt_add2(sum2[0], sum2[1]));
                     lsum += s2.x + s2.y;
@@ -738,7 +723,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     // rows of V that no row of this tile sees but whose page is there: what they hold is not ours to multiply, even by 0
                     const int rows_log = min(a.c.page_log, 7), z0 = k.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
                     pt_wait_warp(&v_full[grp], turn, &abort_flag, a.status, 90);
-                    for (int i = tid & 255; i < (z1 - z0) * 16; i += 256)
+                    for (int i = tid & 127; i < (z1 - z0) * 16; i += 128)
                         *reinterpret_cast<uint4*>(sKV + (size_t)grp * 2 * PT_TILE + PT_TILE + (size_t)((i >> 3) & 1) * PT_BOX + (size_t)(z0 + (i >> 4)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
@@ -746,31 +731,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) pt_arrive(&p_full[grp]);
             }
-            // ---- the segment's rows ----
+            // ---- the segment's rows: a thread half of a row's dims ----
             const int last_t = t0 < n ? t0 + (n - 1 - t0) / 2 * 2 : -1;      // this group's last tile
             if (last_t >= 0) pt_wait_warp(&o_full[grp], (uint32_t)((g0 + last_t) >> 1) & 1u, &abort_flag, a.status, 91);
-            if (part == 0) s_m[grp][row] = m;
-            s_l[grp][part][row] = lsum;
+            s_m[grp][row] = m;
+            s_l[grp][row] = lsum;
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             meet();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float m0 = s_m[0][row], m1 = s_m[1][row], mx = fmaxf(m0, m1);
             const float f0 = m0 == -INFINITY ? 0.f : m0 == mx ? 1.f : pg_ex2(m0 - mx), f1 = m1 == -INFINITY ? 0.f : m1 == mx ? 1.f : pg_ex2(m1 - mx);
-            float sum = (s_l[0][0][row] + s_l[0][1][row]) * f0 + (s_l[1][0][row] + s_l[1][1][row]) * f1;
-            const int dim0 = (warp >> 2) * 32;       // a quarter of the row's dims
-            float o[32];
+            float sum = s_l[0][row] * f0 + s_l[1][row] * f1;
+            const int dim0 = grp * 64;
+            float o[64];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            for (int j = 0; j < 64; ++j) o[j] = 0.f;
             if (n > 0 && live) {
-                uint32_t v[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float f = h ? f1 : f0;
-                    tc_ld32(v, trow + 256u + (uint32_t)(h * 128 + dim0));
+                    uint32_t v[2][32];
+                    tc_ld32(v[0], trow + 256u + (uint32_t)(h * 128 + dim0));
+                    tc_ld32(v[1], trow + 256u + (uint32_t)(h * 128 + dim0 + 32));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (f != 0.f)                    // (a group without a tile, or without a key that the row sees: TMEM may hold anything)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(v[j]), f, o[j]);
+                        for (int j = 0; j < 64; ++j) o[j] = fmaf(__uint_as_float(v[j >> 5][j & 31]), f, o[j]);
                 }
             }
             if (n > 0) {
@@ -782,32 +768,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             if (gave_up) sum = NAN;
             bool bad = !(sum <= FLT_MAX);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) bad = bad || !(fabsf(o[j]) <= FLT_MAX);
+            for (int j = 0; j < 64; ++j) bad = bad || !(fabsf(o[j]) <= FLT_MAX);
             if (bad && row < k.rows && !gave_up) atomicOr(&s_bad[quad], 1u << lane);
             const bool whole = w.whole();
             float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
             const int buf = n_q & 1;
             if (whole) {
                 const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                uint4 pk[4];
+                uint4 pk[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 8; ++j)
                     pk[j] = make_uint4(T::pack(o[8 * j] * r, o[8 * j + 1] * r), T::pack(o[8 * j + 2] * r, o[8 * j + 3] * r), T::pack(o[8 * j + 4] * r, o[8 * j + 5] * r),
                                        T::pack(o[8 * j + 6] * r, o[8 * j + 7] * r));
                 if (n > 0) {
                     // through the place of Q (every product of the segment has completed), so that 16 lanes write a row's 256 bytes; 16-byte chunks XORed by the row
                     uint4* const so = reinterpret_cast<uint4*>(pt_raw + buf * PT_TILE);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) so[row * 16 + ((dim0 / 8 + j) ^ (row & 7))] = pk[j];
+                    for (int j = 0; j < 8; ++j) so[row * 16 + ((dim0 / 8 + j) ^ (row & 7))] = pk[j];
                 } else if (row < k.rows) {           // nothing seen: zeros
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(pg_o_row(a, w.s, row) + dim0 * 2 + j * 16) = pk[j];
+                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(pg_o_row(a, w.s, row) + dim0 * 2 + j * 16) = pk[j];
                 }
             } else if (row < k.rows) {
                 float* const dst = parts + (size_t)row * PG_PART;
                 if (dim0 == 0) *reinterpret_cast<float2*>(dst) = make_float2(gave_up ? NAN : mx, sum);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(dst + 4 + dim0 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(dst + 4 + dim0 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             }
             meet();
             if (whole && n > 0) {
@@ -822,7 +808,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 for (int q = 0; q < 4; ++q)
                     for (unsigned b = s_bad[q]; b; b &= b - 1) {
                         const int rr = q * 32 + __ffs(b) - 1;
-                        pg_redo_row<T, PT_SOFT / 32>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 9);
+                        pg_redo_row<T, PT_WARPS>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 1);
                         if (tid < 64) {
                             const float L = s_res[1], r = L > 0.f || L != L ? 1.f / L : 0.f;
                             if (whole) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, rr) + tid * 4) = T::pack(s_res[4 + 2 * tid] * r, s_res[5 + 2 * tid] * r);
@@ -851,12 +837,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     // After a wait gave up (nobody waits any more): the loads land and the products end before this block's memory and columns are somebody else's.
-    if (warp == PT_SOFT / 32 && abort_flag && lane == 0) {
+    if ((warp == PT_WARPS || warp == PT_WARPS + 1) && abort_flag && lane == 0) {
         for (int i = max(0, armed_q - 2); i < armed_q; ++i) tc_drain(&q_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, armed_k - 2); i < armed_k; ++i) tc_drain(&k_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, armed_v - 2); i < armed_v; ++i) tc_drain(&v_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, armed - 2); i < armed; ++i) tc_drain(warp == PT_WARPS ? &k_full[i & 1] : &v_full[i & 1], (i >> 1) & 1);
     }
-    if (warp == PT_SOFT / 32 + 1) {
+    if (warp == PT_WARPS + 2) {
         if (abort_flag && elect_one()) {
             pt_commit(&drain_bar);
             tc_drain(&drain_bar, 0);
