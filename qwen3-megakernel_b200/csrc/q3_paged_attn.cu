@@ -94,10 +94,11 @@ __device__ __forceinline__ unsigned char* pg_o_row(const PagedAttnArgs& a, const
 
 // A row again, key by key, reading only what it sees: for rows whose result is not finite.  A product adds 0 * v for keys that a row does not see
 // beside those that its tile's later tokens see, and 0 * inf is no number.  Warps of the block take keys in turn (a lane four dims); leaves maximum, sum and
-// output in res[0], res[1], res[4 ..].  `buf` holds 132 floats a warp.  Every thread of the block calls it; ends with a barrier.
-template <typename T, int WARPS>
+// output in res[0], res[1], res[4 ..].  `buf` holds 132 floats a warp.  Every thread of the WARPS warps
+// from FIRST on calls it; ends with their barrier.
+template <typename T, int WARPS, int FIRST>
 __device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment& s, const PgKeys& k, int row, float* buf, float* res, int threads_bar) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - FIRST, tid = threadIdx.x - 32 * FIRST;
     auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "n"(WARPS * 32) : "memory"); };
     const uint2 q2 = *reinterpret_cast<const uint2*>(pg_q_row(a, s, row) + lane * 8);
     const float2 qa = T::unpack(q2.x), qb = T::unpack(q2.y);
@@ -133,13 +134,13 @@ __device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment
             if (mw == -INFINITY) continue;
             const float f = mw == top ? 1.f : pg_ex2(mw - top);
             sum += buf[w * 132 + 1] * f;
-            v += buf[w * 132 + 4 + threadIdx.x] * f;
+            v += buf[w * 132 + 4 + tid] * f;
         }
     }
     sync();
     if (warp < 4) {
-        res[4 + threadIdx.x] = v;
-        if (threadIdx.x == 0) { res[0] = top; res[1] = sum; }
+        res[4 + tid] = v;
+        if (tid == 0) { res[0] = top; res[1] = sum; }
     }
     sync();
 }
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
         __syncthreads();
         for (unsigned bad = s_bad; bad; bad &= bad - 1) {
             const int row = __ffs(bad) - 1;
-            pg_redo_row<T, PR_WARPS>(a, s, k, row, reinterpret_cast<float*>(pr_raw), s_res, 0);
+            pg_redo_row<T, PR_WARPS, 0>(a, s, k, row, reinterpret_cast<float*>(pr_raw), s_res, 0);
             store(row, s_res[0], s_res[1], s_res[4 + tid]);
         }
         __syncthreads();
@@ -384,31 +385,45 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Chunks of new tokens: 128 rows (128 / group tokens of every q head of a kv head) against tiles of 128 keys on tcgen05.mma, accumulators in TMEM.
-//     S  = Q K^T     M 128 x N 128 keys x K 128 dims, both K-major        -> TMEM columns [0, 128) / [128, 256), by the parity of the tile
-//     P  = 2^(S - m) two groups of four warps, a thread a row; group g takes the tiles of parity g, so that one group's exponentials
-//                    run while the tensor pipe and the hand-offs of the other's tile do.  P takes the place of S in TMEM
-//     O += P V       V is the MN-major operand straight from its tile; an O a group -> columns [256, 384) / [384, 512)
+//     S  = Q K^T     M 128 x N 128 keys x K 128 dims, both K-major        -> TMEM columns [128 i, 128 i + 128) of NS buffers
+//     P  = 2^(S - m) two groups of four warps, a thread a row; group g takes the tiles of parity g.  P takes the place of S in TMEM
+//     O += P V       V is the MN-major operand straight from its tile                          -> columns [384, 512) (fp16: an O a group)
 // K and V come page by page (a TMA box a page and half of the dims; a page that is not there, or that no row of the tile sees, lies
-// outside the tensor and reads as zeros), each by a warp of its own, and a block walks the segments of its run without draining: tiles are counted over all of them, the next
-// segment's Q has a buffer of its own, its first scores are under way while the last one's rows are finished.
-// O is rescaled only when a score exceeds the maximum that P is taken under by 2^8.
+// outside the tensor and reads as zeros), each by a warp of its own, S and O are issued by a warp each, and a block walks the segments of its run without draining: tiles are
+// counted over all of them, the next segment's Q has a buffer of its own, its first scores are under way while the last one's rows are finished.
+//
+// bf16: P has fp32's exponents, so that m need not be the maximum: the largest score of the segment's first tile (0 where a row sees none of it) serves all its
+// tiles.  Nothing is rescaled, no other tile is searched for its maximum, one O serves both groups, and there is room for three S: scores run two
+// tiles ahead of the softmax.  A row that leaves fp32's range (scores 88 above the first tile's) is not finite at the end, one that has vanished (no weight
+// above 2^-100 though it sees keys) is seen by its sum: both are done again row by row.  P is truncated to bf16, and its sum is that of the truncated values, which takes
+// the truncation's mean out of the quotient: what is left of it is as large as of rounding (a conversion would be the special-function pipe's, like the exponentials).
+// fp16: P must not leave [2^-24, 2^16), so m follows a group's maximum, and its O is rescaled when a score exceeds m by 2^8; two S and two O.
+//
 // A wait that gives up lets every later one give up at once; all warps still meet at every barrier, rows that are not finished become NaN, and the block drains
 // what is under way before it leaves.
 // ------------------------------------------------------------------------------------------------------------------------------
-constexpr int PT_SOFT = 256, PT_WARPS = PT_SOFT / 32, PT_THREADS = PT_SOFT + 96;      // warps 0..7 softmax and output, 8 TMA of Q and K, 9 TMA of V, 10 MMA and TMEM
+constexpr int PT_SOFT = 256, PT_WARPS = PT_SOFT / 32, PT_THREADS = PT_SOFT + 128;
+constexpr int PT_MMA_O = 0, PT_LOAD_K = 1, PT_LOAD_V = 2, PT_MMA_S = 3, PT_FIRST = 4;      // warps: products with V and TMEM, TMA of Q and K, TMA of V, scores; 4..11 softmax and
+                                                                                           // output (a warp's place in its four is its quarter of the rows)
 constexpr int PT_KEYS = 128;                                  // keys of a tile, the unit of work
 constexpr uint32_t PT_BOX = 128 * 128, PT_TILE = 2 * PT_BOX;  // [128 rows][64 dims] with 128-byte swizzle; 128 x 128
 constexpr size_t PT_SMEM = 2 * PT_TILE + 2 * 2 * PT_TILE;     // two of Q, two stages of K and V
 constexpr float PT_LAG = 8.f;
 
 // The thread looks at the barrier without being parked: a tile has eight hand-offs.
+// PARK: it may sleep up to 20 us between two looks (it wakes when the phase completes).
+template <bool PARK = false>
 __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
     unsigned it = 0;
     unsigned long long t0 = 0;
     for (;;) {
         uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity) : "memory");
+        if constexpr (PARK)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity), "r"(20000u) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity) : "memory");
         if (ok) return true;
         if (*abort_flag) return false;
         if ((++it & 63u) == 0) {
@@ -422,8 +437,9 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
         }
     }
 }
+template <bool PARK = false>
 __device__ __forceinline__ bool pt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
-    return one_lane_waits([&] { return pt_wait(bar, parity, abort_flag, status, site); });
+    return one_lane_waits([&] { return pt_wait<PARK>(bar, parity, abort_flag, status, site); });
 }
 // MN-major operand: rows are keys (the K index), 64 dims a row; the next 64 dims a box further, the next 8 keys 1024 bytes
 __device__ __forceinline__ uint64_t pt_desc_mn(uint32_t smem_addr) {
@@ -472,11 +488,15 @@ __device__ __forceinline__ int pt_tiles(const PgKeys& k) { return (k.key1 - k.ke
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v, const PagedAttnArgs a) {
+    constexpr bool ONE = T::BF;                     // one O, m from the first tile
+    constexpr int NS = ONE ? 3 : 2;                 // buffers of S and P
     extern __shared__ __align__(1024) unsigned char pt_raw[];
     __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PT_THREADS / 32];
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free, drain_bar;
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[NS], p_full[NS], s_free[NS], o_full[2], o_free, drain_bar[2];
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_flag;
+    __shared__ __align__(8) uint64_t ref_full;
+    __shared__ float s_ref[128];                    // ONE: what a row's P of the segment is taken under
     __shared__ float s_m[2][128], s_l[2][128];      // at a segment's end: per group, a row's maximum and sum
     __shared__ unsigned s_bad[4];
     __shared__ float s_res[132];
@@ -496,15 +516,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         for (int s = 0; s < 2; ++s) {
             pt_init(&k_full[s], 1); pt_init(&v_full[s], 1); pt_init(&k_empty[s], 1); pt_init(&v_empty[s], 1);
             pt_init(&q_full[s], 1); pt_init(&q_empty[s], PT_WARPS);
-            pt_init(&s_full[s], 1); pt_init(&p_full[s], 4); pt_init(&o_full[s], 1);
+            pt_init(&o_full[s], 1); pt_init(&drain_bar[s], 1);
         }
+        for (int s = 0; s < NS; ++s) { pt_init(&s_full[s], 1); pt_init(&p_full[s], 4); pt_init(&s_free[s], 1); }
         pt_init(&o_free, PT_WARPS);
-        pt_init(&drain_bar, 1);
+        pt_init(&ref_full, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
         s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
     }
-    if (warp == PT_WARPS + 2) {
+    if (warp == PT_MMA_O) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base_s)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -516,9 +537,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const long long from = pg_run_start(total, blocks, blockIdx.x), to = pg_run_start(total, blocks, blockIdx.x + 1);
 
     int armed = 0, armed_q = 0;                     // tiles of K (V) and of Q that this warp has requested
-    if (warp == PT_WARPS || warp == PT_WARPS + 1) {
+    if (warp == PT_LOAD_K || warp == PT_LOAD_V) {
         // ---------------------------------------------------------------------- TMA: a lane a box
-        const bool is_v = warp != PT_WARPS;
+        const bool is_v = warp == PT_LOAD_V;
         const int rows_log = min(a.c.page_log, 7), boxes = PT_KEYS >> rows_log, j = lane >> 1, half = lane & 1;      // a page's rows are cut into boxes of 128 at most
         const bool mine = j < boxes;
         const CUtensorMap* const map = is_v ? &tm_v : &tm_k;
@@ -536,7 +557,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             int next = n > 0 ? entry(0) : -1;
             if (n > 0 && !is_v) {
                 const int buf = n_q & 1;
-                if (n_q >= 2 && !pt_wait_warp(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) break;
+                if (n_q >= 2 && !pt_wait_warp<true>(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) break;
                 if (lane == 0) {
                     pt_expect(&q_full[buf], PT_TILE);
 #pragma unroll
@@ -551,7 +572,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 const int s = g & 1, slot = (key0 + t * PT_KEYS) & ((1 << a.c.page_log) - 1);
                 const int page = (unsigned)next < (unsigned)a.c.n_pages ? next : a.c.n_pages;      // no such page: outside the tensor
                 if (t + 1 < n) next = entry(t + 1);  // (on its way while this tile is waited for)
-                ok = g < 2 || pt_wait_warp(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
+                ok = g < 2 || pt_wait_warp<true>(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
                 if (!ok) break;
                 if (lane == 0) pt_expect(&full[s], PT_TILE);
                 __syncwarp();
@@ -562,80 +583,77 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             }
             ok = ok && w.next(a.sh, qs, kl);
         }
-    } else if (warp == PT_WARPS + 2) {
-        // ---------------------------------------------------------------------- MMA issuer
+    } else if (warp == PT_MMA_S) {
+        // ---------------------------------------------------------------------- scores
         if (elect_one()) {
-            const uint32_t idesc_s = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), idesc_o = idesc_s | (1u << 16);
+            constexpr uint32_t idesc = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             constexpr uint64_t BOX = PT_BOX >> 4, TILE = PT_TILE >> 4;
-            const uint64_t dq = tc_desc(tc_smem(pt_raw)), dk = tc_desc(tc_smem(sKV)), dv = pt_desc_mn(tc_smem(sKV + PT_TILE));
-            // two walks over the same tiles: scores run two tiles ahead of the products with V
-            PgWalk ws, wp;
-            int gs = 0, ts = -1, ns = 0, q_s = -1;   // the tile whose scores come next: number, place in its segment, tiles of that, segments with tiles before it
-            auto next_s = [&]() -> bool {            // the next tile of ws, if there is one
-                if (ts + 1 < ns) { ++ts; return true; }
-                for (;;) {
-                    if (!(ts < 0 ? ws.begin(a.sh, s_prefix, qs, kl, from, to) : ws.next(a.sh, qs, kl))) return false;
-                    ns = pt_tiles(pg_keys(a, ws.s));
-                    ts = 0;
-                    if (ns > 0) { ++q_s; return true; }
-                }
-            };
-            auto issue_s = [&]() -> bool {
-                const int s = gs & 1, buf = q_s & 1;
-                if (ts == 0 && !pt_wait(&q_full[buf], (q_s >> 1) & 1, &abort_flag, a.status, 83)) return false;
-                if (!pt_wait(&k_full[s], (gs >> 1) & 1, &abort_flag, a.status, 84)) return false;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t dqs = dq + (uint64_t)buf * TILE, dks = dk + (uint64_t)s * 2 * TILE;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {        // 16 dims a step: four steps a box
-                    const uint64_t o = (uint64_t)(k >> 2) * BOX + (uint64_t)(k & 3) * 2;
-                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-                                 ::"r"(tmem_base + (uint32_t)s * 128u), "l"(dqs + o), "l"(dks + o), "r"(idesc_s), "r"(k ? 1u : 0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
-                }
-                pt_commit(&s_full[s]);
-                pt_commit(&k_empty[s]);
-                ++gs;
-                return true;
-            };
-            bool more = next_s();
-            bool ok = true;
-            for (int i = 0; i < 2 && more && ok; ++i) {
-                ok = issue_s();
-                more = ok && next_s();
-            }
-            int g = 0, seg = 0;
-            bool left = ok && wp.begin(a.sh, s_prefix, qs, kl, from, to);
-            while (left && ok) {
-                const int n = pt_tiles(pg_keys(a, wp.s));
-                for (int t = 0; t < n && ok; ++t, ++g) {
-                    const int b = g & 1;
-                    if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
-                    ok = ok && pt_wait(&v_full[b], (g >> 1) & 1, &abort_flag, a.status, 87) && pt_wait(&p_full[b], (g >> 1) & 1, &abort_flag, a.status, 86);
+            const uint64_t dq = tc_desc(tc_smem(pt_raw)), dk = tc_desc(tc_smem(sKV));
+            PgWalk w;
+            bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
+            int g = 0, n_q = 0, b = 0, use = 0;      // tile, segments with tiles, buffer of S and how often it has been used
+            while (ok) {
+                const int n = pt_tiles(pg_keys(a, w.s));
+                for (int t = 0; t < n; ++t, ++g) {
+                    const int s = g & 1, buf = n_q & 1;
+                    if (t == 0) ok = pt_wait(&q_full[buf], (n_q >> 1) & 1, &abort_flag, a.status, 83);
+                    ok = ok && pt_wait(&k_full[s], (g >> 1) & 1, &abort_flag, a.status, 84);
+                    if (use > 0) ok = ok && pt_wait(&s_free[b], (use - 1) & 1, &abort_flag, a.status, 92);      // P of the tile before in this buffer has been multiplied
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t dvs = dv + (uint64_t)b * 2 * TILE;
-                    const uint32_t tp = tmem_base + (uint32_t)b * 128u;
+                    const uint64_t dqs = dq + (uint64_t)buf * TILE, dks = dk + (uint64_t)s * 2 * TILE;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {    // 16 dims a step: four steps a box
+                        const uint64_t o = (uint64_t)(k >> 2) * BOX + (uint64_t)(k & 3) * 2;
+                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+                                     ::"r"(tmem_base + (uint32_t)b * 128u), "l"(dqs + o), "l"(dks + o), "r"(idesc), "r"(k ? 1u : 0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+                    }
+                    pt_commit(&s_full[b]);
+                    pt_commit(&k_empty[s]);
+                    if (++b == NS) { b = 0; ++use; }
+                }
+                if (n > 0) ++n_q;
+                ok = ok && w.next(a.sh, qs, kl);
+            }
+        }
+    } else if (warp == PT_MMA_O) {
+        // ---------------------------------------------------------------------- products with V
+        if (elect_one()) {
+            constexpr uint32_t idesc = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint64_t TILE = PT_TILE >> 4;
+            const uint64_t dv = pt_desc_mn(tc_smem(sKV + PT_TILE));
+            PgWalk w;
+            bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
+            int g = 0, seg = 0, b = 0, use = 0;
+            while (ok) {
+                const int n = pt_tiles(pg_keys(a, w.s));
+                for (int t = 0; t < n; ++t, ++g) {
+                    const int s = g & 1;
+                    if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
+                    ok = ok && pt_wait(&v_full[s], (g >> 1) & 1, &abort_flag, a.status, 87) && pt_wait(&p_full[b], use & 1, &abort_flag, a.status, 86);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t dvs = dv + (uint64_t)s * 2 * TILE;
+                    const uint32_t tp = tmem_base + (uint32_t)b * 128u, to_o = tmem_base + (ONE ? 384u : 256u + (uint32_t)s * 128u);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)      // 16 keys a step: eight columns of P (two a column)
                         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-                                     ::"r"(tp + 256u), "r"(tp + (uint32_t)k * 8u), "l"(dvs + (uint64_t)k * (2048 >> 4)), "r"(idesc_o), "r"((t >= 2 || k) ? 1u : 0u),
+                                     ::"r"(to_o), "r"(tp + (uint32_t)k * 8u), "l"(dvs + (uint64_t)k * (2048 >> 4)), "r"(idesc), "r"((t >= (ONE ? 1 : 2) || k) ? 1u : 0u),
                                        "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
-                    pt_commit(&o_full[b]);
-                    pt_commit(&v_empty[b]);
-                    if (more) {                      // over P of this tile: the pipe works in order
-                        ok = issue_s();
-                        more = ok && next_s();
-                    }
+                    pt_commit(&s_free[b]);
+                    pt_commit(&v_empty[s]);
+                    if (!ONE) pt_commit(&o_full[s]);
+                    else if (t == n - 1) pt_commit(&o_full[0]);
+                    if (++b == NS) { b = 0; ++use; }
                 }
                 if (n > 0) ++seg;
-                left = wp.next(a.sh, qs, kl);
+                ok = ok && w.next(a.sh, qs, kl);
             }
         }
-    } else {
+    } else if (warp >= PT_FIRST) {
         // ---------------------------------------------------------------------- softmax and output: row = TMEM lane
-        const int quad = warp & 3, row = quad * 32 + lane, grp = warp >> 2;
+        const int quad = warp & 3, row = quad * 32 + lane, grp = (warp >> 2) - 1, st = tid - 32 * PT_FIRST;
         const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
-        const uint32_t ts = trow + (uint32_t)(grp * 128), to_o = trow + 256u + (uint32_t)(grp * 128);
         auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(PT_SOFT) : "memory"); };
         PgWalk w;
         bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
@@ -656,64 +674,106 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 return __ballot_sync(0xffffffffu, key >= k.key1 || pg_page(a.c, w.s.b, key) >= 0) & 0xffu;
             };
             for (int t = t0; t < n; t += 2) {
-                const int g = g0 + t, tile0 = k.key0 + t * PT_KEYS;
-                const uint32_t turn = (uint32_t)(g >> 1) & 1u;
+                const int g = g0 + t, tile0 = k.key0 + t * PT_KEYS, b = g % NS;
+                const uint32_t turn = (uint32_t)(g >> 1) & 1u, ts = trow + (uint32_t)b * 128u;
                 const unsigned pages = every ? 0xffu : pages_of(tile0);
-                pt_wait_warp(&s_full[grp], turn, &abort_flag, a.status, 88);
+                const bool masked = tile0 + PT_KEYS - 1 > k.qpos0 || tile0 + PT_KEYS > k.key1 || pages != 0xffu;
+                pt_wait_warp(&s_full[b], (uint32_t)(g / NS) & 1u, &abort_flag, a.status, 88);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                auto hide = [&](uint32_t (&r)[32], int h) {              // what the row does not see of the tile's quarter h
+                    const int most = last - tile0 - h * 32;
+                    const unsigned gone = ~(pages >> (h * 2));
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j > most || ((gone >> (j >> 4)) & 1u)) r[j] = 0xff800000u;            // -inf
+                };
                 if (live) {
-                    uint32_t r[4][32];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) tc_ld32(r[h], ts + (uint32_t)(h * 32));
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (tile0 + PT_KEYS - 1 > k.qpos0 || tile0 + PT_KEYS > k.key1 || pages != 0xffu) {
-                        const int most = last - tile0;
-                        const unsigned gone = ~pages;
-#pragma unroll
-                        for (int h = 0; h < 4; ++h)
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (h * 32 + j > most || ((gone >> (h * 2 + (j >> 4))) & 1u)) r[h][j] = 0xff800000u;            // -inf
-                    }
-                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2)
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) x[h] = pt_max3(x[h], r[h][j], r[h][j + 1]);
-                    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
-                    const bool raise = !(top <= m + PT_LAG);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
-                        if (raise) m = top;
-                        lsum *= c;
-                        if (t >= 2) {                // O of the segment's tiles so far, once the last of them has been added
-                            pt_wait_warp(&o_full[grp], turn ^ 1u, &abort_flag, a.status, 89);
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (!ONE || t == 0) {
+                        float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                            for (int h = 0; h < 128; h += 16) {
-                                uint32_t o[16];
-                                tc_ld16(o, to_o + (uint32_t)h);
-                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t r[32];
+                            tc_ld32(r, ts + (uint32_t)(h * 32));
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            if (masked) hide(r, h);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
-                                pt_st16(to_o + (uint32_t)h, o);
+                            for (int j = 0; j < 32; j += 4) { x[0] = pt_max3(x[0], r[j], r[j + 1]); x[1] = pt_max3(x[1], r[j + 2], r[j + 3]); }
+                        }
+                        const float top = fmaxf(x[0], x[1]) * a.scale;
+                        if constexpr (ONE) {
+                            m = top == -INFINITY ? 0.f : top;
+                            s_ref[row] = m;
+                        } else {
+                            const bool raise = !(top <= m + PT_LAG);
+                            if (__any_sync(0xffffffffu, raise)) {
+                                const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
+                                if (raise) m = top;
+                                lsum *= c;
+                                if (t >= 2) {        // O of the group's tiles so far, once the last of them has been added
+                                    pt_wait_warp(&o_full[grp], turn ^ 1u, &abort_flag, a.status, 89);
+                                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                                    for (int h = 0; h < 128; h += 16) {
+                                        uint32_t o[16];
+                                        tc_ld16(o, trow + 256u + (uint32_t)(grp * 128 + h));
+                                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
+                                        pt_st16(trow + 256u + (uint32_t)(grp * 128 + h), o);
+                                    }
+                                }
                             }
                         }
                     }
+                }
+                if constexpr (ONE) {                 // the group of the first tile leaves its m to the other
+                    if (t == 0) {
+                        __syncwarp();
+                        if (lane == 0) pt_arrive(&ref_full);
+                    } else if (t == 1) {
+                        pt_wait_warp(&ref_full, (uint32_t)n_q & 1u, &abort_flag, a.status, 93);
+                        m = s_ref[row];
+                    }
+                }
+                if (live) {
                     const float ms = m == -INFINITY ? 0.f : m;               // (nothing seen so far: every exponential is 0)
                     const uint64_t c2 = pt_pair(a.scale, a.scale), m2 = pt_pair(-ms, -ms);
                     uint64_t sum2[2] = {0ull, 0ull};                         // (two elements an instruction where it is one of the FMA pipe's)
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    auto weigh = [&](const uint32_t (&r)[32], int h) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float2 x2 = pt_unpair(pt_fma2(pt_pair(__uint_as_float(r[h][2 * j]), __uint_as_float(r[h][2 * j + 1])), c2, m2));
+                            const float2 x2 = pt_unpair(pt_fma2(pt_pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2, m2));
                             const float e0 = pg_ex2(x2.x), e1 = pg_ex2(x2.y);
-                            sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(e0, e1));
-                            pk[j] = T::pack(e0, e1);
+                            if constexpr (ONE) {
+                                pk[j] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
+                                sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(__uint_as_float(__float_as_uint(e0) & 0xffff0000u), __uint_as_float(__float_as_uint(e1) & 0xffff0000u)));
+                            } else {
+                                pk[j] = T::pack(e0, e1);
+                                sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(e0, e1));
+                            }
                         }
-                        pt_st16(ts + (uint32_t)(h * 16), pk);
+                        pt_st16(ts + (uint32_t)(h * 16), pk);                // (over scores that have been read)
+                    };
+                    if (!masked) {
+                        uint32_t r[2][32];
+                        tc_ld32(r[0], ts);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            if (h < 3) tc_ld32(r[(h + 1) & 1], ts + (uint32_t)(h * 32 + 32));
+                            weigh(r[h & 1], h);
+                            if (h < 3) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t r[32];
+                            tc_ld32(r, ts + (uint32_t)(h * 32));
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            hide(r, h);
+                            weigh(r, h);
+                        }
                     }
                     const float2 s2 = pt_unpair(pt_add2(sum2[0], sum2[1]));
                     lsum += s2.x + s2.y;
@@ -723,40 +783,58 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     // rows of V that no row of this tile sees but whose page is there: what they hold is not ours to multiply, even by 0
                     const int rows_log = min(a.c.page_log, 7), z0 = k.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
                     pt_wait_warp(&v_full[grp], turn, &abort_flag, a.status, 90);
-                    for (int i = tid & 127; i < (z1 - z0) * 16; i += 128)
+                    for (int i = st & 127; i < (z1 - z0) * 16; i += 128)
                         *reinterpret_cast<uint4*>(sKV + (size_t)grp * 2 * PT_TILE + PT_TILE + (size_t)((i >> 3) & 1) * PT_BOX + (size_t)(z0 + (i >> 4)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) pt_arrive(&p_full[grp]);
+                if (lane == 0) pt_arrive(&p_full[b]);
             }
             // ---- the segment's rows: a thread half of a row's dims ----
-            const int last_t = t0 < n ? t0 + (n - 1 - t0) / 2 * 2 : -1;      // this group's last tile
-            if (last_t >= 0) pt_wait_warp(&o_full[grp], (uint32_t)((g0 + last_t) >> 1) & 1u, &abort_flag, a.status, 91);
-            s_m[grp][row] = m;
+            if constexpr (ONE) {
+                if (n > 0) pt_wait_warp(&o_full[0], (uint32_t)n_q & 1u, &abort_flag, a.status, 91);
+            } else {
+                const int last_t = t0 < n ? t0 + (n - 1 - t0) / 2 * 2 : -1;  // this group's last tile
+                if (last_t >= 0) pt_wait_warp(&o_full[grp], (uint32_t)((g0 + last_t) >> 1) & 1u, &abort_flag, a.status, 91);
+                s_m[grp][row] = m;
+            }
             s_l[grp][row] = lsum;
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             meet();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float m0 = s_m[0][row], m1 = s_m[1][row], mx = fmaxf(m0, m1);
-            const float f0 = m0 == -INFINITY ? 0.f : m0 == mx ? 1.f : pg_ex2(m0 - mx), f1 = m1 == -INFINITY ? 0.f : m1 == mx ? 1.f : pg_ex2(m1 - mx);
-            float sum = s_l[0][row] * f0 + s_l[1][row] * f1;
             const int dim0 = grp * 64;
-            float o[64];
-#pragma unroll
-            for (int j = 0; j < 64; ++j) o[j] = 0.f;
-            if (n > 0 && live) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float f = h ? f1 : f0;
-                    uint32_t v[2][32];
-                    tc_ld32(v[0], trow + 256u + (uint32_t)(h * 128 + dim0));
-                    tc_ld32(v[1], trow + 256u + (uint32_t)(h * 128 + dim0 + 32));
+            float mx, sum, o[64];
+            if constexpr (ONE) {
+                mx = n > 0 ? s_ref[row] : -INFINITY;
+                sum = s_l[0][row] + s_l[1][row];
+                uint32_t v[2][32];
+                if (n > 0 && live) {
+                    tc_ld32(v[0], trow + 384u + (uint32_t)dim0);
+                    tc_ld32(v[1], trow + 384u + (uint32_t)(dim0 + 32));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (f != 0.f)                    // (a group without a tile, or without a key that the row sees: TMEM may hold anything)
+                }
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) o[j] = fmaf(__uint_as_float(v[j >> 5][j & 31]), f, o[j]);
+                for (int j = 0; j < 64; ++j) o[j] = n > 0 && live ? __uint_as_float(v[j >> 5][j & 31]) : 0.f;
+            } else {
+                const float m0 = s_m[0][row], m1 = s_m[1][row];
+                mx = fmaxf(m0, m1);
+                const float f0 = m0 == -INFINITY ? 0.f : m0 == mx ? 1.f : pg_ex2(m0 - mx), f1 = m1 == -INFINITY ? 0.f : m1 == mx ? 1.f : pg_ex2(m1 - mx);
+                sum = s_l[0][row] * f0 + s_l[1][row] * f1;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) o[j] = 0.f;
+                if (n > 0 && live) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float f = h ? f1 : f0;
+                        uint32_t v[2][32];
+                        tc_ld32(v[0], trow + 256u + (uint32_t)(h * 128 + dim0));
+                        tc_ld32(v[1], trow + 256u + (uint32_t)(h * 128 + dim0 + 32));
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (f != 0.f)                // (a group without a tile, or without a key that the row sees: TMEM may hold anything)
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) o[j] = fmaf(__uint_as_float(v[j >> 5][j & 31]), f, o[j]);
+                    }
                 }
             }
             if (n > 0) {
@@ -766,7 +844,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             }
             const bool gave_up = abort_flag;
             if (gave_up) sum = NAN;
-            bool bad = !(sum <= FLT_MAX);
+            bool bad = !(sum <= FLT_MAX) || (ONE && n > 0 && last >= k.key0 && sum < 7.9e-31f);      // (2^-100)
 #pragma unroll
             for (int j = 0; j < 64; ++j) bad = bad || !(fabsf(o[j]) <= FLT_MAX);
             if (bad && row < k.rows && !gave_up) atomicOr(&s_bad[quad], 1u << lane);
@@ -790,6 +868,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(pg_o_row(a, w.s, row) + dim0 * 2 + j * 16) = pk[j];
                 }
             } else if (row < k.rows) {
+                if (ONE && sum > 0.f && sum <= FLT_MAX) {      // as if taken under about the row's own maximum: the sum between 1 and 4
+                    const int e = min(max((int)(__float_as_uint(sum) >> 23) - 127, -126), 126);
+                    const float f = __uint_as_float((unsigned)(127 - e) << 23);
+                    sum *= f; mx += (float)e;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) o[j] *= f;
+                }
                 float* const dst = parts + (size_t)row * PG_PART;
                 if (dim0 == 0) *reinterpret_cast<float2*>(dst) = make_float2(gave_up ? NAN : mx, sum);
 #pragma unroll
@@ -798,7 +883,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             meet();
             if (whole && n > 0) {
                 const uint4* const so = reinterpret_cast<const uint4*>(pt_raw + buf * PT_TILE);
-                for (int i = tid; i < k.rows * 16; i += PT_SOFT) {
+                for (int i = st; i < k.rows * 16; i += PT_SOFT) {
                     const int rr = i >> 4, c = i & 15;
                     *reinterpret_cast<uint4*>(pg_o_row(a, w.s, rr) + c * 16) = so[rr * 16 + (c ^ (rr & 7))];
                 }
@@ -808,19 +893,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 for (int q = 0; q < 4; ++q)
                     for (unsigned b = s_bad[q]; b; b &= b - 1) {
                         const int rr = q * 32 + __ffs(b) - 1;
-                        pg_redo_row<T, PT_WARPS>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 1);
-                        if (tid < 64) {
+                        pg_redo_row<T, PT_WARPS, PT_FIRST>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 1);
+                        if (st < 64) {
                             const float L = s_res[1], r = L > 0.f || L != L ? 1.f / L : 0.f;
-                            if (whole) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, rr) + tid * 4) = T::pack(s_res[4 + 2 * tid] * r, s_res[5 + 2 * tid] * r);
+                            if (whole) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, rr) + st * 4) = T::pack(s_res[4 + 2 * st] * r, s_res[5 + 2 * st] * r);
                             else {
                                 float* const dst = parts + (size_t)rr * PG_PART;
-                                dst[4 + 2 * tid] = s_res[4 + 2 * tid]; dst[5 + 2 * tid] = s_res[5 + 2 * tid];
-                                if (tid == 0) { dst[0] = s_res[0]; dst[1] = L; }
+                                dst[4 + 2 * st] = s_res[4 + 2 * st]; dst[5 + 2 * st] = s_res[5 + 2 * st];
+                                if (st == 0) { dst[0] = s_res[0]; dst[1] = L; }
                             }
                         }
                     }
                 meet();
-                if (tid < 4) s_bad[tid] = 0;
+                if (st < 4) s_bad[st] = 0;
             }
             if (n > 0) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -829,7 +914,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 ++n_q;
             }
             g0 += n;
-            if (tid == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
+            if (st == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
             first = false;
             left = w.next(a.sh, qs, kl);
         }
@@ -837,16 +922,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     // After a wait gave up (nobody waits any more): the loads land and the products end before this block's memory and columns are somebody else's.
-    if ((warp == PT_WARPS || warp == PT_WARPS + 1) && abort_flag && lane == 0) {
+    if ((warp == PT_LOAD_K || warp == PT_LOAD_V) && abort_flag && lane == 0) {
         for (int i = max(0, armed_q - 2); i < armed_q; ++i) tc_drain(&q_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, armed - 2); i < armed; ++i) tc_drain(warp == PT_WARPS ? &k_full[i & 1] : &v_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, armed - 2); i < armed; ++i) tc_drain(warp == PT_LOAD_K ? &k_full[i & 1] : &v_full[i & 1], (i >> 1) & 1);
     }
-    if (warp == PT_WARPS + 2) {
-        if (abort_flag && elect_one()) {
-            pt_commit(&drain_bar);
-            tc_drain(&drain_bar, 0);
-        }
-        __syncwarp();
+    if ((warp == PT_MMA_O || warp == PT_MMA_S) && abort_flag && elect_one()) {
+        pt_commit(&drain_bar[warp == PT_MMA_S]);
+        tc_drain(&drain_bar[warp == PT_MMA_S], 0);
+    }
+    __syncthreads();
+    if (warp == PT_MMA_O) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
