@@ -94,12 +94,11 @@ __device__ __forceinline__ unsigned char* pg_o_row(const PagedAttnArgs& a, const
 
 // A row again, key by key, reading only what it sees: for rows whose result is not finite.  A product adds 0 * v for keys that a row does not see
 // beside those that its tile's later tokens see, and 0 * inf is no number.  Warps of the block take keys in turn (a lane four dims); leaves maximum, sum and
-// output in res[0], res[1], res[4 ..].  `buf` holds 132 floats a warp.  Every thread of the WARPS warps
-// from FIRST on calls it; ends with their barrier.
-template <typename T, int WARPS, int FIRST>
-__device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment& s, const PgKeys& k, int row, float* buf, float* res, int threads_bar) {
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - FIRST, tid = threadIdx.x - 32 * FIRST;
-    auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "n"(WARPS * 32) : "memory"); };
+// output in res[0], res[1], res[4 ..].  `buf` holds 132 floats a warp.  Every thread of WARPS warps
+// calls it, `warp` is its place among them; `sync` is their barrier, and the last thing done.
+template <typename T, int WARPS, typename Sync>
+__device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment& s, const PgKeys& k, int row, int warp, float* buf, float* res, const Sync& sync) {
+    const int lane = threadIdx.x & 31, tid = warp * 32 + lane;
     const uint2 q2 = *reinterpret_cast<const uint2*>(pg_q_row(a, s, row) + lane * 8);
     const float2 qa = T::unpack(q2.x), qb = T::unpack(q2.y);
     const int end = min(k.key1, k.qpos0 + (row >> a.group_log) + 1);
@@ -165,7 +164,7 @@ __device__ __forceinline__ uint32_t pg_transpose(uint32_t w) {
 }
 
 template <typename T, int NB>
-__global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int COLS = 8 * NB, LD = 132;
     constexpr int PL = NB <= 2 ? 2 : 1;               // planes of P: two where the products have room beside the bytes
     static_assert(COLS * LD * 4 <= PR_STAGES * PR_STAGE, "a warp's outputs fit its stages");
@@ -369,9 +368,12 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
             if (!(fabsf(v) <= FLT_MAX && L <= FLT_MAX)) atomicOr(&s_bad, 1u << row);
         }
         __syncthreads();
+        auto sync = [] { __syncthreads(); };
         for (unsigned bad = s_bad; bad; bad &= bad - 1) {
             const int row = __ffs(bad) - 1;
-            pg_redo_row<T, PR_WARPS, 0>(a, s, k, row, reinterpret_cast<float*>(pr_raw), s_res, 0);
+            const PgSegment seg = s;                 // (copies: what a call is handed by address would live in memory all along)
+            const PgKeys keys = k;
+            pg_redo_row<T, PR_WARPS>(a, seg, keys, row, warp, reinterpret_cast<float*>(pr_raw), s_res, sync);
             store(row, s_res[0], s_res[1], s_res[4 + tid]);
         }
         __syncthreads();
@@ -386,25 +388,31 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const PagedAt
 // ------------------------------------------------------------------------------------------------------------------------------
 // Chunks of new tokens: 128 rows (128 / group tokens of every q head of a kv head) against tiles of 128 keys on tcgen05.mma, accumulators in TMEM.
 //     S  = Q K^T     M 128 x N 128 keys x K 128 dims, both K-major        -> TMEM columns [128 i, 128 i + 128) of NS buffers
-//     P  = 2^(S - m) two groups of four warps, a thread a row; group g takes the tiles of parity g.  P takes the place of S in TMEM
+//     P  = 2^(S - m) NS groups of four warps, a thread a row, take turns at the tiles: a group a buffer.  P takes the place of S in TMEM
 //     O += P V       V is the MN-major operand straight from its tile                          -> columns [384, 512) (fp16: an O a group)
 // K and V come page by page (a TMA box a page and half of the dims; a page that is not there, or that no row of the tile sees, lies
-// outside the tensor and reads as zeros), each by a warp of its own, S and O are issued by a warp each, and a block walks the segments of its run without draining: tiles are
-// counted over all of them, the next segment's Q has a buffer of its own, its first scores are under way while the last one's rows are finished.
+// outside the tensor and reads as zeros), each by a warp of its own, S and O are issued by a warp each.  A block walks the segments of its run without draining: the warp that
+// loads K works them out ahead of the others (code that runs once a segment comes from far away: 4000 clocks where every warp walked for itself), tiles are counted over all
+// of them, the next segment's Q has a buffer of its own, its first scores are under way while the last one's rows are finished.
 //
 // bf16: P has fp32's exponents, so that m need not be the maximum: the largest score of the segment's first tile (0 where a row sees none of it) serves all its
-// tiles.  Nothing is rescaled, no other tile is searched for its maximum, one O serves both groups, and there is room for three S: scores run two
-// tiles ahead of the softmax.  A row that leaves fp32's range (scores 88 above the first tile's) is not finite at the end, one that has vanished (no weight
+// tiles.  Nothing is rescaled, no other tile is searched for its maximum, one O serves all groups, and there is room for three S.  A row that leaves fp32's range (scores 88 above the first tile's) is not finite at the end, one that has vanished (no weight
 // above 2^-100 though it sees keys) is seen by its sum: both are done again row by row.  P is truncated to bf16, and its sum is that of the truncated values, which takes
 // the truncation's mean out of the quotient: what is left of it is as large as of rounding (a conversion would be the special-function pipe's, like the exponentials).
 // fp16: P must not leave [2^-24, 2^16), so m follows a group's maximum, and its O is rescaled when a score exceeds m by 2^8; two S and two O.
 //
-// A wait that gives up lets every later one give up at once; all warps still meet at every barrier, rows that are not finished become NaN, and the block drains
-// what is under way before it leaves.
+// A wait that gives up lets every later one give up at once (those in which the softmax warps meet are waits like the others); the block then drains what is under way and
+// leaves NaN in all rows of its run.
 // ------------------------------------------------------------------------------------------------------------------------------
-constexpr int PT_SOFT = 256, PT_WARPS = PT_SOFT / 32, PT_THREADS = PT_SOFT + 128;
-constexpr int PT_MMA_O = 0, PT_LOAD_K = 1, PT_LOAD_V = 2, PT_MMA_S = 3, PT_FIRST = 4;      // warps: products with V and TMEM, TMA of Q and K, TMA of V, scores; 4..11 softmax and
+constexpr int PT_MMA_O = 0, PT_LOAD_K = 1, PT_LOAD_V = 2, PT_MMA_S = 3, PT_FIRST = 4;      // warps: products with V and TMEM, TMA of Q and K, TMA of V, scores; from 4 on softmax and
                                                                                            // output (a warp's place in its four is its quarter of the rows)
+template <typename T> struct PtShape {
+    static constexpr bool ONE = T::BF;                        // one O, m from the first tile
+    static constexpr int NS = ONE ? 3 : 2;                    // buffers of S and P
+};
+constexpr int PT_RING = 4;                                    // segments that have been worked out ahead
+constexpr int PT_GROUPS = 2, PT_THREADS = 32 * PT_FIRST + PT_GROUPS * 128;
+struct PtSeg { int n, b, h, q_row, key0, key1, qpos0, rows, whole, every; };      // n tiles of one item's keys; n < 0: the run is over
 constexpr int PT_KEYS = 128;                                  // keys of a tile, the unit of work
 constexpr uint32_t PT_BOX = 128 * 128, PT_TILE = 2 * PT_BOX;  // [128 rows][64 dims] with 128-byte swizzle; 128 x 128
 constexpr size_t PT_SMEM = 2 * PT_TILE + 2 * 2 * PT_TILE;     // two of Q, two stages of K and V
@@ -483,22 +491,44 @@ __device__ __forceinline__ void pt_arrive(uint64_t* bar) { asm volatile("mbarrie
 __device__ __forceinline__ void pt_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc_smem(bar)) : "memory");
 }
-__device__ __forceinline__ int pt_tiles(const PgKeys& k) { return (k.key1 - k.key0 + PT_KEYS - 1) / PT_KEYS; }
+
+// How a group of four softmax warps waits: one lane looks at the barrier, the others sleep at a named barrier (a look takes 100 clocks of the barrier unit: twelve
+// warps that looked for themselves saw finished scores 1500 clocks late).  The four warps take every decision together, so they always meet again.
+struct PtGroup {
+    int grp, quad, lane;
+    volatile int* abort_flag;
+    uint32_t* status;
+    __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, 128;" ::"r"(2 + grp) : "memory"); }
+    __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, uint32_t site) const {
+        if (quad == 0 && lane == 0) pt_wait(bar, parity, abort_flag, status, site);
+        __syncwarp();
+        sync();
+    }
+};
+// the group's own, for pg_redo_row
+struct PtSync {
+    const PtGroup& group;
+    __device__ __forceinline__ void operator()() const { group.sync(); }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                                                                   const __grid_constant__ CUtensorMap tm_v, const PagedAttnArgs a) {
-    constexpr bool ONE = T::BF;                     // one O, m from the first tile
-    constexpr int NS = ONE ? 3 : 2;                 // buffers of S and P
+                                                                            const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
+    using S = PtShape<T>;
+    constexpr bool ONE = S::ONE;
+    constexpr int NS = S::NS, GROUPS = PT_GROUPS;
     extern __shared__ __align__(1024) unsigned char pt_raw[];
     __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PT_THREADS / 32];
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[NS], p_full[NS], s_free[NS], o_full[2], o_free, drain_bar[2];
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[NS], p_full[NS], s_free[NS], o_full[2], o_free, ref_full, l_full[2], drain_bar[2];
+    __shared__ __align__(8) uint64_t seg_full[PT_RING], seg_empty[PT_RING];
+    __shared__ PtSeg s_seg[PT_RING];
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_flag;
-    __shared__ __align__(8) uint64_t ref_full;
-    __shared__ float s_ref[128];                    // ONE: what a row's P of the segment is taken under
-    __shared__ float s_m[2][128], s_l[2][128];      // at a segment's end: per group, a row's maximum and sum
-    __shared__ unsigned s_bad[4];
+    __shared__ float s_ref[2][128];                 // ONE: what a row's P is taken under, by the segment's parity
+    __shared__ float s_m[2][128], s_l[2][128];      // what the group that does not write a segment's rows leaves to the other: maximum (fp16) and sum, by the segment's parity
+    __shared__ float s_room[4 * 132];               // of pg_redo_row
+    __shared__ unsigned s_bad[GROUPS][4];           // per group: rows that are done again
+    __shared__ int s_ok[GROUPS];                      // per group: what its first warp has decided for all four
     __shared__ float s_res[132];
 
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
@@ -515,15 +545,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
             pt_init(&k_full[s], 1); pt_init(&v_full[s], 1); pt_init(&k_empty[s], 1); pt_init(&v_empty[s], 1);
-            pt_init(&q_full[s], 1); pt_init(&q_empty[s], PT_WARPS);
+            pt_init(&q_full[s], 1); pt_init(&q_empty[s], 1); pt_init(&l_full[s], 4);
             pt_init(&o_full[s], 1); pt_init(&drain_bar[s], 1);
         }
         for (int s = 0; s < NS; ++s) { pt_init(&s_full[s], 1); pt_init(&p_full[s], 4); pt_init(&s_free[s], 1); }
-        pt_init(&o_free, PT_WARPS);
+        for (int s = 0; s < PT_RING; ++s) { pt_init(&seg_full[s], 1); pt_init(&seg_empty[s], 3 + 4 * GROUPS); }
+        pt_init(&o_free, 4);
         pt_init(&ref_full, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
-        s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
+        for (int e = 0; e < 4 * GROUPS; ++e) s_bad[e >> 2][e & 3] = 0;
     }
     if (warp == PT_MMA_O) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base_s)), "r"(512u) : "memory");
@@ -536,6 +567,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     const int *qs = a.c.q_start, *kl = a.c.kv_len;
     const long long from = pg_run_start(total, blocks, blockIdx.x), to = pg_run_start(total, blocks, blockIdx.x + 1);
 
+    // segment number i as the loader of K has worked it out; n < 0 at the run's end, or after a wait gave up.  One thread, or a warp.
+    auto segment = [&](int i) {
+        PtSeg d;
+        d.n = -1;
+        if (pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 95)) {
+            d = s_seg[i % PT_RING];
+            pt_arrive(&seg_empty[i % PT_RING]);
+        }
+        return d;
+    };
+    auto segment_warp = [&](int i) {
+        PtSeg d;
+        d.n = -1;
+        if (pt_wait_warp<true>(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 95)) {
+            d = s_seg[i % PT_RING];
+            __syncwarp();
+            if (lane == 0) pt_arrive(&seg_empty[i % PT_RING]);
+        }
+        return d;
+    };
+
     int armed = 0, armed_q = 0;                     // tiles of K (V) and of Q that this warp has requested
     if (warp == PT_LOAD_K || warp == PT_LOAD_V) {
         // ---------------------------------------------------------------------- TMA: a lane a box
@@ -545,43 +597,70 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         const CUtensorMap* const map = is_v ? &tm_v : &tm_k;
         uint64_t *const full = is_v ? v_full : k_full, *const empty = is_v ? v_empty : k_empty;
         const uint32_t dst0 = tc_smem(sKV + (is_v ? PT_TILE : 0)) + (uint32_t)half * PT_BOX + ((uint32_t)j << (rows_log + 7));
-        PgWalk w;
-        bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
         int g = 0, n_q = 0;
-        while (ok) {
-            const PgKeys k = pg_keys(a, w.s);
-            const int n = pt_tiles(k), key0 = k.key0 + (j << rows_log);
-            const int* const table = a.c.table + (long long)w.s.b * a.c.table_stride;
+        auto load = [&](const PtSeg& d) -> bool {
+            const int key0 = d.key0 + (j << rows_log);
+            const int* const table = a.c.table + (long long)d.b * a.c.table_stride;
             // the page of this lane's box of tile t, as the table has it
-            auto entry = [&](int t) { const int key = key0 + t * PT_KEYS; return mine && key < k.key1 ? table[key >> a.c.page_log] : -1; };
-            int next = n > 0 ? entry(0) : -1;
-            if (n > 0 && !is_v) {
+            auto entry = [&](int t) { const int key = key0 + t * PT_KEYS; return mine && key < d.key1 ? table[key >> a.c.page_log] : -1; };
+            int next = d.n > 0 ? entry(0) : -1;
+            if (d.n > 0 && !is_v) {
                 const int buf = n_q & 1;
-                if (n_q >= 2 && !pt_wait_warp<true>(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) break;
+                if (n_q >= 2 && !pt_wait_warp<true>(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) return false;
                 if (lane == 0) {
                     pt_expect(&q_full[buf], PT_TILE);
 #pragma unroll
                     for (int b = 0; b < 2; ++b)       // rows past q are zeros
                         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                     ::"r"(tc_smem(pt_raw + buf * PT_TILE + b * PT_BOX)), "l"(&tm_q), "r"(64 * b), "r"(w.s.h << a.group_log), "r"(w.s.seq.q0 + (w.s.r << a.sh.tile_log)),
+                                     ::"r"(tc_smem(pt_raw + buf * PT_TILE + b * PT_BOX)), "l"(&tm_q), "r"(64 * b), "r"(d.h << a.group_log), "r"(d.q_row),
                                        "r"(tc_smem(&q_full[buf])) : "memory");
                 }
                 armed_q = ++n_q;
             }
-            for (int t = 0; t < n; ++t, ++g) {
+            for (int t = 0; t < d.n; ++t, ++g) {
                 const int s = g & 1, slot = (key0 + t * PT_KEYS) & ((1 << a.c.page_log) - 1);
                 const int page = (unsigned)next < (unsigned)a.c.n_pages ? next : a.c.n_pages;      // no such page: outside the tensor
-                if (t + 1 < n) next = entry(t + 1);  // (on its way while this tile is waited for)
-                ok = g < 2 || pt_wait_warp<true>(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81);
-                if (!ok) break;
+                if (t + 1 < d.n) next = entry(t + 1);  // (on its way while this tile is waited for)
+                if (g >= 2 && !pt_wait_warp<true>(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81)) return false;
                 if (lane == 0) pt_expect(&full[s], PT_TILE);
                 __syncwarp();
                 if (mine)
                     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                                 ::"r"(dst0 + (uint32_t)s * 2u * PT_TILE), "l"(map), "r"(64 * half), "r"(slot), "r"(w.s.h), "r"(page), "r"(tc_smem(&full[s])) : "memory");
+                                 ::"r"(dst0 + (uint32_t)s * 2u * PT_TILE), "l"(map), "r"(64 * half), "r"(slot), "r"(d.h), "r"(page), "r"(tc_smem(&full[s])) : "memory");
                 armed = g + 1;
             }
-            ok = ok && w.next(a.sh, qs, kl);
+            return true;
+        };
+        if (is_v) {
+            for (int i = 0;; ++i) {
+                const PtSeg d = segment_warp(i);
+                if (d.n < 0 || !load(d)) break;
+            }
+        } else {
+            PgWalk w;
+            bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
+            for (int i = 0;; ++i) {
+                PtSeg d;
+                d.n = -1;
+                if (left) {
+                    const PgKeys k = pg_keys(a, w.s);
+                    d = PtSeg{(k.key1 - k.key0 + PT_KEYS - 1) / PT_KEYS, w.s.b, w.s.h, w.s.seq.q0 + (w.s.r << a.sh.tile_log), k.key0, k.key1, k.qpos0, k.rows, w.whole(), 1};
+                    bool every = true;               // all pages of the segment are there
+                    for (int e = (k.key0 >> a.c.page_log) + lane; d.n > 0 && e <= (k.key1 - 1) >> a.c.page_log; e += 32)
+                        every = every && (unsigned)a.c.table[(long long)d.b * a.c.table_stride + e] < (unsigned)a.c.n_pages;
+                    d.every = __all_sync(0xffffffffu, every);
+                }
+                if (i >= PT_RING && !pt_wait_warp<true>(&seg_empty[i % PT_RING], (uint32_t)(i / PT_RING - 1) & 1u, &abort_flag, a.status, 96)) break;
+                if (lane == 0) {
+                    s_seg[i % PT_RING] = d;
+                    pt_arrive(&seg_full[i % PT_RING]);
+                }
+                __syncwarp();
+                if (d.n < 0 || !load(d)) break;
+                if (lane == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
+                first = false;
+                left = w.next(a.sh, qs, kl);
+            }
         }
     } else if (warp == PT_MMA_S) {
         // ---------------------------------------------------------------------- scores
@@ -589,11 +668,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             constexpr uint32_t idesc = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             constexpr uint64_t BOX = PT_BOX >> 4, TILE = PT_TILE >> 4;
             const uint64_t dq = tc_desc(tc_smem(pt_raw)), dk = tc_desc(tc_smem(sKV));
-            PgWalk w;
-            bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
-            int g = 0, n_q = 0, b = 0, use = 0;      // tile, segments with tiles, buffer of S and how often it has been used
-            while (ok) {
-                const int n = pt_tiles(pg_keys(a, w.s));
+            bool ok = true;
+            for (int i = 0, g = 0, n_q = 0, b = 0, use = 0; ok; ++i) {       // tile, segments with tiles, buffer of S and how often it has been used
+                const int n = segment(i).n;
+                if (n < 0) break;
                 for (int t = 0; t < n; ++t, ++g) {
                     const int s = g & 1, buf = n_q & 1;
                     if (t == 0) ok = pt_wait(&q_full[buf], (n_q >> 1) & 1, &abort_flag, a.status, 83);
@@ -610,10 +688,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     }
                     pt_commit(&s_full[b]);
                     pt_commit(&k_empty[s]);
+                    if (t == n - 1) pt_commit(&q_empty[buf]);
                     if (++b == NS) { b = 0; ++use; }
                 }
                 if (n > 0) ++n_q;
-                ok = ok && w.next(a.sh, qs, kl);
             }
         }
     } else if (warp == PT_MMA_O) {
@@ -622,11 +700,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             constexpr uint32_t idesc = (1u << 4) | (T::BF ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             constexpr uint64_t TILE = PT_TILE >> 4;
             const uint64_t dv = pt_desc_mn(tc_smem(sKV + PT_TILE));
-            PgWalk w;
-            bool ok = w.begin(a.sh, s_prefix, qs, kl, from, to);
-            int g = 0, seg = 0, b = 0, use = 0;
-            while (ok) {
-                const int n = pt_tiles(pg_keys(a, w.s));
+            bool ok = true;
+            for (int i = 0, g = 0, seg = 0, b = 0, use = 0; ok; ++i) {
+                const int n = segment(i).n;
+                if (n < 0) break;
                 for (int t = 0; t < n; ++t, ++g) {
                     const int s = g & 1;
                     if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
@@ -634,7 +711,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t dvs = dv + (uint64_t)s * 2 * TILE;
-                    const uint32_t tp = tmem_base + (uint32_t)b * 128u, to_o = tmem_base + (ONE ? 384u : 256u + (uint32_t)s * 128u);
+                    const uint32_t tp = tmem_base + (uint32_t)b * 128u, to_o = tmem_base + (ONE ? 384u : 256u + (uint32_t)b * 128u);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)      // 16 keys a step: eight columns of P (two a column)
                         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
@@ -642,97 +719,96 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                                        "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
                     pt_commit(&s_free[b]);
                     pt_commit(&v_empty[s]);
-                    if (!ONE) pt_commit(&o_full[s]);
+                    if (!ONE) pt_commit(&o_full[b]);
                     else if (t == n - 1) pt_commit(&o_full[0]);
                     if (++b == NS) { b = 0; ++use; }
                 }
                 if (n > 0) ++seg;
-                ok = ok && w.next(a.sh, qs, kl);
             }
         }
-    } else if (warp >= PT_FIRST) {
+    } else {
         // ---------------------------------------------------------------------- softmax and output: row = TMEM lane
         const int quad = warp & 3, row = quad * 32 + lane, grp = (warp >> 2) - 1, st = tid - 32 * PT_FIRST;
         const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
-        auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(PT_SOFT) : "memory"); };
-        PgWalk w;
-        bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
-        int g0 = 0, n_q = 0;
-        while (left) {
-            const PgKeys k = pg_keys(a, w.s);
-            const int n = pt_tiles(k);
-            const int last = min(k.qpos0 + (row >> a.group_log), k.key1 - 1);       // the last key this row sees
-            const bool live = quad * 32 < k.rows;                            // (the warp has a row)
-            const int t0 = (grp ^ g0) & 1;
+        const PtGroup group{grp, quad, lane, &abort_flag, a.status};
+        bool first = true;
+        int g0 = 0, n_q = 0;                         // number of the segment's first tile; segments with tiles
+        for (int i = 0;; ++i) {
+            if (quad == 0 && lane == 0) s_ok[grp] = pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 97);
+            __syncwarp();
+            group.sync();
+            if (!s_ok[grp]) break;
+            const PtSeg d = s_seg[i % PT_RING];
+            __syncwarp();
+            if (lane == 0) pt_arrive(&seg_empty[i % PT_RING]);
+            const int n = d.n;
+            if (n < 0) break;
+            const int last = min(d.qpos0 + (row >> a.group_log), d.key1 - 1);       // the last key this row sees
+            const bool live = quad * 32 < d.rows;                            // (the warp has a row)
+            const int t0 = (grp + GROUPS - g0 % GROUPS) % GROUPS;            // this group's first tile
             float m = -INFINITY, lsum = 0.f;
-            // whether all pages of the segment are there (usually), and which of a tile's are: bit i for the keys 16 i ..
-            bool every = true;
-            for (int i = (k.key0 >> a.c.page_log) + lane; n > 0 && i <= (k.key1 - 1) >> a.c.page_log; i += 32) every = every && (unsigned)a.c.table[(long long)w.s.b * a.c.table_stride + i] < (unsigned)a.c.n_pages;
-            every = __all_sync(0xffffffffu, every);
-            auto pages_of = [&](int tile0) {
+            auto pages_of = [&](int tile0) {         // bit i: whether the keys 16 i .. of a tile have a page (or nobody sees them)
                 const int key = tile0 + 16 * (lane & 7);
-                return __ballot_sync(0xffffffffu, key >= k.key1 || pg_page(a.c, w.s.b, key) >= 0) & 0xffu;
+                return __ballot_sync(0xffffffffu, key >= d.key1 || pg_page(a.c, d.b, key) >= 0) & 0xffu;
             };
-            for (int t = t0; t < n; t += 2) {
-                const int g = g0 + t, tile0 = k.key0 + t * PT_KEYS, b = g % NS;
-                const uint32_t turn = (uint32_t)(g >> 1) & 1u, ts = trow + (uint32_t)b * 128u;
-                const unsigned pages = every ? 0xffu : pages_of(tile0);
-                const bool masked = tile0 + PT_KEYS - 1 > k.qpos0 || tile0 + PT_KEYS > k.key1 || pages != 0xffu;
-                pt_wait_warp(&s_full[b], (uint32_t)(g / NS) & 1u, &abort_flag, a.status, 88);
+            for (int t = t0; t < n; t += GROUPS) {
+                const int g = g0 + t, tile0 = d.key0 + t * PT_KEYS, b = g % NS;
+                const uint32_t ts = trow + (uint32_t)b * 128u;
+                const unsigned pages = d.every ? 0xffu : pages_of(tile0);
+                const bool masked = tile0 + PT_KEYS - 1 > d.qpos0 || tile0 + PT_KEYS > d.key1 || pages != 0xffu;
+                group.wait(&s_full[b], (uint32_t)(g / NS) & 1u, 88);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                auto hide = [&](uint32_t (&r)[32], int h) {              // what the row does not see of the tile's quarter h
+                auto hide = [&](uint32_t (&r)[32], int h) {                  // what the row does not see of the tile's quarter h
                     const int most = last - tile0 - h * 32;
                     const unsigned gone = ~(pages >> (h * 2));
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (j > most || ((gone >> (j >> 4)) & 1u)) r[j] = 0xff800000u;            // -inf
                 };
-                if (live) {
-                    if (!ONE || t == 0) {
-                        float x[2] = {-INFINITY, -INFINITY};
+                if (live && (!ONE || t == 0)) {
+                    float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                        for (int h = 0; h < 4; ++h) {
-                            uint32_t r[32];
-                            tc_ld32(r, ts + (uint32_t)(h * 32));
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                            if (masked) hide(r, h);
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t r[32];
+                        tc_ld32(r, ts + (uint32_t)(h * 32));
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (masked) hide(r, h);
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) { x[0] = pt_max3(x[0], r[j], r[j + 1]); x[1] = pt_max3(x[1], r[j + 2], r[j + 3]); }
-                        }
-                        const float top = fmaxf(x[0], x[1]) * a.scale;
-                        if constexpr (ONE) {
-                            m = top == -INFINITY ? 0.f : top;
-                            s_ref[row] = m;
-                        } else {
-                            const bool raise = !(top <= m + PT_LAG);
-                            if (__any_sync(0xffffffffu, raise)) {
-                                const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
-                                if (raise) m = top;
-                                lsum *= c;
-                                if (t >= 2) {        // O of the group's tiles so far, once the last of them has been added
-                                    pt_wait_warp(&o_full[grp], turn ^ 1u, &abort_flag, a.status, 89);
-                                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        for (int j = 0; j < 32; j += 4) { x[0] = pt_max3(x[0], r[j], r[j + 1]); x[1] = pt_max3(x[1], r[j + 2], r[j + 3]); }
+                    }
+                    const float top = fmaxf(x[0], x[1]) * a.scale;
+                    if constexpr (ONE) {
+                        m = top == -INFINITY ? 0.f : top;
+                        s_ref[n_q & 1][row] = m;
+                    } else {
+                        const bool raise = !(top <= m + PT_LAG);
+                        if (__any_sync(0xffffffffu, raise)) {
+                            const float c = raise ? pg_ex2(m - top) : 1.f;       // (m of -inf: 0)
+                            if (raise) m = top;
+                            lsum *= c;
+                            if (t >= GROUPS) {       // O of the group's tiles so far, once the last of them has been added
+                                pt_wait_warp(&o_full[grp], (uint32_t)((g >> 1) - 1) & 1u, &abort_flag, a.status, 89);      // (not every warp of the group comes here)
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                                    for (int h = 0; h < 128; h += 16) {
-                                        uint32_t o[16];
-                                        tc_ld16(o, trow + 256u + (uint32_t)(grp * 128 + h));
-                                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                                for (int h = 0; h < 128; h += 16) {
+                                    uint32_t o[16];
+                                    tc_ld16(o, trow + 256u + (uint32_t)(grp * 128 + h));
+                                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
-                                        pt_st16(trow + 256u + (uint32_t)(grp * 128 + h), o);
-                                    }
+                                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * c);
+                                    pt_st16(trow + 256u + (uint32_t)(grp * 128 + h), o);
                                 }
                             }
                         }
                     }
                 }
-                if constexpr (ONE) {                 // the group of the first tile leaves its m to the other
+                if constexpr (ONE) {                 // the group of the first tile leaves its m to the others
                     if (t == 0) {
                         __syncwarp();
                         if (lane == 0) pt_arrive(&ref_full);
-                    } else if (t == 1) {
-                        pt_wait_warp(&ref_full, (uint32_t)n_q & 1u, &abort_flag, a.status, 93);
-                        m = s_ref[row];
+                    } else if (t == t0) {
+                        group.wait(&ref_full, (uint32_t)n_q & 1u, 93);
+                        m = s_ref[n_q & 1][row];
                     }
                 }
                 if (live) {
@@ -779,159 +855,189 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     lsum += s2.x + s2.y;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                if (tile0 + PT_KEYS > k.key1) {
+                if (tile0 + PT_KEYS > d.key1) {
                     // rows of V that no row of this tile sees but whose page is there: what they hold is not ours to multiply, even by 0
-                    const int rows_log = min(a.c.page_log, 7), z0 = k.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
-                    pt_wait_warp(&v_full[grp], turn, &abort_flag, a.status, 90);
-                    for (int i = st & 127; i < (z1 - z0) * 16; i += 128)
-                        *reinterpret_cast<uint4*>(sKV + (size_t)grp * 2 * PT_TILE + PT_TILE + (size_t)((i >> 3) & 1) * PT_BOX + (size_t)(z0 + (i >> 4)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    const int rows_log = min(a.c.page_log, 7), z0 = d.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
+                    group.wait(&v_full[g & 1], (uint32_t)(g >> 1) & 1u, 90);
+                    for (int e = st & 127; e < (z1 - z0) * 16; e += 128)
+                        *reinterpret_cast<uint4*>(sKV + (size_t)(g & 1) * 2 * PT_TILE + PT_TILE + (size_t)((e >> 3) & 1) * PT_BOX + (size_t)(z0 + (e >> 4)) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) pt_arrive(&p_full[b]);
             }
-            // ---- the segment's rows: a thread half of a row's dims ----
-            if constexpr (ONE) {
-                if (n > 0) pt_wait_warp(&o_full[0], (uint32_t)n_q & 1u, &abort_flag, a.status, 91);
-            } else {
-                const int last_t = t0 < n ? t0 + (n - 1 - t0) / 2 * 2 : -1;  // this group's last tile
-                if (last_t >= 0) pt_wait_warp(&o_full[grp], (uint32_t)((g0 + last_t) >> 1) & 1u, &abort_flag, a.status, 91);
-                s_m[grp][row] = m;
-            }
-            s_l[grp][row] = lsum;
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            meet();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int dim0 = grp * 64;
-            float mx, sum, o[64];
-            if constexpr (ONE) {
-                mx = n > 0 ? s_ref[row] : -INFINITY;
-                sum = s_l[0][row] + s_l[1][row];
-                uint32_t v[2][32];
-                if (n > 0 && live) {
-                    tc_ld32(v[0], trow + 384u + (uint32_t)dim0);
-                    tc_ld32(v[1], trow + 384u + (uint32_t)(dim0 + 32));
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                }
-#pragma unroll
-                for (int j = 0; j < 64; ++j) o[j] = n > 0 && live ? __uint_as_float(v[j >> 5][j & 31]) : 0.f;
-            } else {
-                const float m0 = s_m[0][row], m1 = s_m[1][row];
-                mx = fmaxf(m0, m1);
-                const float f0 = m0 == -INFINITY ? 0.f : m0 == mx ? 1.f : pg_ex2(m0 - mx), f1 = m1 == -INFINITY ? 0.f : m1 == mx ? 1.f : pg_ex2(m1 - mx);
-                sum = s_l[0][row] * f0 + s_l[1][row] * f1;
-#pragma unroll
-                for (int j = 0; j < 64; ++j) o[j] = 0.f;
-                if (n > 0 && live) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float f = h ? f1 : f0;
-                        uint32_t v[2][32];
-                        tc_ld32(v[0], trow + 256u + (uint32_t)(h * 128 + dim0));
-                        tc_ld32(v[1], trow + 256u + (uint32_t)(h * 128 + dim0 + 32));
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        if (f != 0.f)                // (a group without a tile, or without a key that the row sees: TMEM may hold anything)
-#pragma unroll
-                            for (int j = 0; j < 64; ++j) o[j] = fmaf(__uint_as_float(v[j >> 5][j & 31]), f, o[j]);
-                    }
-                }
-            }
-            if (n > 0) {
+            // ---- the segment's rows: the groups write in turn, the other goes on to the next segment's tiles ----
+            const int par = i & 1;
+            if (par != grp) {
+                s_l[par][row] = lsum;
+                if (!ONE) s_m[par][row] = m;
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) pt_arrive(&o_free);
-            }
-            const bool gave_up = abort_flag;
-            if (gave_up) sum = NAN;
-            bool bad = !(sum <= FLT_MAX) || (ONE && n > 0 && last >= k.key0 && sum < 7.9e-31f);      // (2^-100)
+                if (lane == 0) pt_arrive(&l_full[par]);
+            } else {
+                group.wait(&l_full[par], (uint32_t)(i >> 1) & 1u, 94);
+                if constexpr (ONE) {
+                    if (n > 0) group.wait(&o_full[0], (uint32_t)n_q & 1u, 91);
+                } else {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) bad = bad || !(fabsf(o[j]) <= FLT_MAX);
-            if (bad && row < k.rows && !gave_up) atomicOr(&s_bad[quad], 1u << lane);
-            const bool whole = w.whole();
-            float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
-            const int buf = n_q & 1;
-            if (whole) {
-                const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                uint4 pk[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    pk[j] = make_uint4(T::pack(o[8 * j] * r, o[8 * j + 1] * r), T::pack(o[8 * j + 2] * r, o[8 * j + 3] * r), T::pack(o[8 * j + 4] * r, o[8 * j + 5] * r),
-                                       T::pack(o[8 * j + 6] * r, o[8 * j + 7] * r));
-                if (n > 0) {
-                    // through the place of Q (every product of the segment has completed), so that 16 lanes write a row's 256 bytes; 16-byte chunks XORed by the row
-                    uint4* const so = reinterpret_cast<uint4*>(pt_raw + buf * PT_TILE);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) so[row * 16 + ((dim0 / 8 + j) ^ (row & 7))] = pk[j];
-                } else if (row < k.rows) {           // nothing seen: zeros
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(pg_o_row(a, w.s, row) + dim0 * 2 + j * 16) = pk[j];
+                    for (int e = 0; e < 2; ++e) {                            // the last tile of either group
+                        const int te = (e + 2 - (g0 & 1)) & 1;
+                        if (te < n) group.wait(&o_full[e], (uint32_t)((g0 + te + (n - 1 - te) / 2 * 2) >> 1) & 1u, 91);
+                    }
                 }
-            } else if (row < k.rows) {
-                if (ONE && sum > 0.f && sum <= FLT_MAX) {      // as if taken under about the row's own maximum: the sum between 1 and 4
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const bool whole = d.whole != 0;
+                float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
+                float mx, sum, f[2] = {1.f, 0.f};    // the row's m and sum; what the groups' O are multiplied by (ONE: the one's)
+                if constexpr (ONE) {
+                    mx = n > 0 ? s_ref[n_q & 1][row] : -INFINITY;
+                    sum = lsum + s_l[par][row];
+                } else {
+                    const float me[2] = {grp == 0 ? m : s_m[par][row], grp == 0 ? s_m[par][row] : m}, le[2] = {grp == 0 ? lsum : s_l[par][row], grp == 0 ? s_l[par][row] : lsum};
+                    mx = fmaxf(me[0], me[1]);
+                    sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        f[e] = me[e] == -INFINITY ? 0.f : me[e] == mx ? 1.f : pg_ex2(me[e] - mx);
+                        sum += le[e] * f[e];
+                    }
+                }
+                bool bad = !(sum <= FLT_MAX) || (ONE && n > 0 && last >= d.key0 && sum < 7.9e-31f);      // (2^-100)
+                float r = 1.f;                       // the last factor: the sum's inverse, or what makes the sum of a partial result lie between 1 and 4
+                if (whole) {
+                    r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                } else if (ONE && sum > 0.f && sum <= FLT_MAX) {
                     const int e = min(max((int)(__float_as_uint(sum) >> 23) - 127, -126), 126);
-                    const float f = __uint_as_float((unsigned)(127 - e) << 23);
-                    sum *= f; mx += (float)e;
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) o[j] *= f;
+                    r = __uint_as_float((unsigned)(127 - e) << 23);
+                    sum *= r; mx += (float)e;
                 }
-                float* const dst = parts + (size_t)row * PG_PART;
-                if (dim0 == 0) *reinterpret_cast<float2*>(dst) = make_float2(gave_up ? NAN : mx, sum);
+                // (a partial result's maxima and sums lie behind its outputs, [32 quarters of 16 bytes][128 rows])
+                if (!whole && row < d.rows) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(mx, sum);
+                unsigned char* const o_row = a.out + (long long)(d.q_row + (row >> a.group_log)) * a.o_token + (long long)((d.h << a.group_log) + (row & ((1 << a.group_log) - 1))) * a.o_head;
+                uint64_t odd = 0ull;                 // 0, or NaN once an output is not finite
+                if (live) {
+#pragma unroll 1
+                    for (int e = 0; e < HEAD_DIM; e += 32) {
+                        uint64_t o[16];
+                        if (n > 0) {
+                            uint32_t v[32];
+                            tc_ld32(v, trow + (ONE ? 384u : 256u) + (uint32_t)e);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            // (a group without a tile, or without a key that the row sees, has a factor of 0: TMEM may hold anything there)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) *reinterpret_cast<float4*>(dst + 4 + dim0 + 4 * j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-            }
-            meet();
-            if (whole && n > 0) {
-                const uint4* const so = reinterpret_cast<const uint4*>(pt_raw + buf * PT_TILE);
-                for (int i = st; i < k.rows * 16; i += PT_SOFT) {
-                    const int rr = i >> 4, c = i & 15;
-                    *reinterpret_cast<uint4*>(pg_o_row(a, w.s, rr) + c * 16) = so[rr * 16 + (c ^ (rr & 7))];
-                }
-            }
-            if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) {
-                meet();                              // (rows have been written, the buffer of Q is free)
-                for (int q = 0; q < 4; ++q)
-                    for (unsigned b = s_bad[q]; b; b &= b - 1) {
-                        const int rr = q * 32 + __ffs(b) - 1;
-                        pg_redo_row<T, PT_WARPS, PT_FIRST>(a, w.s, k, rr, reinterpret_cast<float*>(pt_raw + buf * PT_TILE), s_res, 1);
-                        if (st < 64) {
-                            const float L = s_res[1], r = L > 0.f || L != L ? 1.f / L : 0.f;
-                            if (whole) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, rr) + st * 4) = T::pack(s_res[4 + 2 * st] * r, s_res[5 + 2 * st] * r);
-                            else {
-                                float* const dst = parts + (size_t)rr * PG_PART;
-                                dst[4 + 2 * st] = s_res[4 + 2 * st]; dst[5 + 2 * st] = s_res[5 + 2 * st];
-                                if (st == 0) { dst[0] = s_res[0]; dst[1] = L; }
+                            for (int j = 0; j < 16; ++j)
+                                o[j] = ONE ? pt_pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]))
+                                           : f[0] != 0.f ? pt_pair(__uint_as_float(v[2 * j]) * f[0], __uint_as_float(v[2 * j + 1]) * f[0]) : 0ull;
+                            if constexpr (!ONE) {
+                                tc_ld32(v, trow + 384u + (uint32_t)e);
+                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                                if (f[1] != 0.f)
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) o[j] = pt_fma2(pt_pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), pt_pair(f[1], f[1]), o[j]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = 0ull;
+                        }
+                        if (e == HEAD_DIM - 32 && n > 0) {       // O has been read
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) pt_arrive(&o_free);
+                        }
+                        const uint64_t r2 = pt_pair(r, r);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            odd = pt_fma2(o[j], 0ull, odd);
+                            o[j] = pt_fma2(o[j], r2, 0x8000000080000000ull);      // (minus zero: added to anything it changes nothing)
+                        }
+                        if (row < d.rows) {
+                            if (!whole) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float2 lo = pt_unpair(o[2 * j]), hi = pt_unpair(o[2 * j + 1]);
+                                    reinterpret_cast<float4*>(parts)[(e / 4 + j) * 128 + row] = make_float4(lo.x, lo.y, hi.x, hi.y);
+                                }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    uint32_t pk[4];
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q) { const float2 x = pt_unpair(o[4 * j + q]); pk[q] = T::pack(x.x, x.y); }
+                                    *reinterpret_cast<uint4*>(o_row + e * 2 + j * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                                }
                             }
                         }
                     }
-                meet();
-                if (st < 4) s_bad[st] = 0;
+                } else if (n > 0) {
+                    __syncwarp();
+                    if (lane == 0) pt_arrive(&o_free);
+                }
+                const float2 odd2 = pt_unpair(odd);
+                bad = (bad || odd2.x != 0.f || odd2.y != 0.f) && row < d.rows;
+                const unsigned again = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0) s_bad[grp][quad] = again;
+                __syncwarp();
+                group.sync();
+                if (s_bad[grp][0] | s_bad[grp][1] | s_bad[grp][2] | s_bad[grp][3]) {
+                    PgSegment seg{};                 // (what pg_redo_row asks of it)
+                    seg.b = d.b; seg.h = d.h; seg.seq.q0 = d.q_row;
+                    const PgKeys keys{d.key0, d.key1, d.qpos0, d.rows};
+                    PtSync sync{group};
+                    for (int q = 0; q < 4; ++q)
+                        for (unsigned b = s_bad[grp][q]; b; b &= b - 1) {
+                            const int rr = q * 32 + __ffs(b) - 1;
+                            // (the groups write in turn: a segment's rows are finished before the next one's are looked at, so one room serves both)
+                            pg_redo_row<T, 4>(a, seg, keys, rr, quad, s_room, s_res, sync);
+                            const int dim = quad * 32 + lane;
+                            const float L = s_res[1], inv = L > 0.f || L != L ? 1.f / L : 0.f, x = s_res[4 + dim], up = __shfl_down_sync(0xffffffffu, x, 1);
+                            if (whole) {
+                                if (!(dim & 1)) *reinterpret_cast<uint32_t*>(pg_o_row(a, seg, rr) + dim * 2) = T::pack(x * inv, up * inv);
+                            } else {
+                                parts[((dim >> 2) * 128 + rr) * 4 + (dim & 3)] = x;
+                                if (dim == 0) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[rr] = make_float2(s_res[0], L);
+                            }
+                            group.sync();
+                        }
+                }
             }
             if (n > 0) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) pt_arrive(&q_empty[buf]);
                 ++n_q;
+                g0 += n;
             }
-            g0 += n;
-            if (st == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
             first = false;
-            left = w.next(a.sh, qs, kl);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    // After a wait gave up (nobody waits any more): the loads land and the products end before this block's memory and columns are somebody else's.
-    if ((warp == PT_LOAD_K || warp == PT_LOAD_V) && abort_flag && lane == 0) {
-        for (int i = max(0, armed_q - 2); i < armed_q; ++i) tc_drain(&q_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, armed - 2); i < armed; ++i) tc_drain(warp == PT_LOAD_K ? &k_full[i & 1] : &v_full[i & 1], (i >> 1) & 1);
+    if (abort_flag) {
+        // A wait gave up (nobody waits any more): the loads land and the products end before this block's memory and columns are somebody else's, and no row of the run
+        // passes for finished.
+        if ((warp == PT_LOAD_K || warp == PT_LOAD_V) && lane == 0) {
+            for (int i = max(0, armed_q - 2); i < armed_q; ++i) tc_drain(&q_full[i & 1], (i >> 1) & 1);
+            for (int i = max(0, armed - 2); i < armed; ++i) tc_drain(warp == PT_LOAD_K ? &k_full[i & 1] : &v_full[i & 1], (i >> 1) & 1);
+        }
+        if ((warp == PT_MMA_O || warp == PT_MMA_S) && elect_one()) {
+            pt_commit(&drain_bar[warp == PT_MMA_S]);
+            tc_drain(&drain_bar[warp == PT_MMA_S], 0);
+        }
+        __syncthreads();
+        PgWalk w;
+        bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
+        while (left) {
+            const int rows = pg_keys(a, w.s).rows;
+            float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
+            for (int e = tid; e < rows * 64; e += PT_THREADS) {
+                if (w.whole()) *reinterpret_cast<uint32_t*>(pg_o_row(a, w.s, e >> 6) + (e & 63) * 4) = 0x7fff7fffu;
+                else if ((e & 63) == 0) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[e >> 6] = make_float2(NAN, NAN);
+            }
+            if (tid == 0 && w.at + w.s.k1 - w.s.k0 >= w.end) pg_leave_cut(a, w, first, total, blocks);
+            first = false;
+            left = w.next(a.sh, qs, kl);
+        }
     }
-    if ((warp == PT_MMA_O || warp == PT_MMA_S) && abort_flag && elect_one()) {
-        pt_commit(&drain_bar[warp == PT_MMA_S]);
-        tc_drain(&drain_bar[warp == PT_MMA_S], 0);
-    }
-    __syncthreads();
     if (warp == PT_MMA_O) {
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
@@ -988,6 +1094,51 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
         const float r = L > 0.f || L != L ? 1.f / L : 0.f;
         *reinterpret_cast<uint2*>(pg_o_row(a, s, row) + lane * 8) = make_uint2(T::pack(v.x * r, v.y * r), T::pack(v.z * r, v.w * r));
     }
+}
+
+// The same for results of the tile kernel, whose outputs lie [32 quarters of 16 bytes][128 rows] with the maxima and sums behind them: a lane a row, a warp eight quarters.
+template <typename T>
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_tiles_kernel(const PagedAttnArgs a) {
+    pdl_launch();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * 8, block = blockIdx.x, row = blockIdx.y * 32 + lane;
+    const int4 cut = *reinterpret_cast<const int4*>(&a.cuts[block]);
+    const int parts = cut.x;
+    if (parts == 0) return;
+    PgSegment s;
+    s.b = cut.z; s.h = cut.w; s.r = a.cuts[block].r;
+    s.seq = pg_seq(a.sh, a.c.q_start, a.c.kv_len, s.b);
+    const int live = min(1 << a.sh.tile_log, s.seq.q - (s.r << a.sh.tile_log)) << a.group_log;
+    if (row >= live) return;
+    auto part = [&](int i) { return a.part + (size_t)(2 * (block + i) + (i == 0 ? cut.y : 0)) * 128 * PG_PART; };
+    auto stats = [&](int i) { return reinterpret_cast<const float2*>(part(i) + 128 * HEAD_DIM)[row]; };
+    float M = -INFINITY;
+    bool nan = false;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) { const float x = stats(i).x; M = fmaxf(M, x); nan = nan || x != x; }
+    if (nan) M = NAN;
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = stats(i);
+        float4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = reinterpret_cast<const float4*>(part(i))[(d0 + j) * 128 + row];
+        const float w = ml.x == -INFINITY ? 0.f : ml.x == Ms ? 1.f : pg_ex2(ml.x - Ms);
+        if (w != 0.f) {
+            L = fmaf(ml.y, w, L);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { v[j].x = fmaf(x[j].x, w, v[j].x); v[j].y = fmaf(x[j].y, w, v[j].y); v[j].z = fmaf(x[j].z, w, v[j].z); v[j].w = fmaf(x[j].w, w, v[j].w); }
+        }
+    }
+    const float r = L > 0.f || L != L ? 1.f / L : 0.f;
+    unsigned char* const out = pg_o_row(a, s, row) + d0 * 8;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        *reinterpret_cast<uint4*>(out + j * 8) = make_uint4(T::pack(v[j].x * r, v[j].y * r), T::pack(v[j].z * r, v[j].w * r), T::pack(v[j + 1].x * r, v[j + 1].y * r), T::pack(v[j + 1].z * r, v[j + 1].w * r));
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
@@ -1057,7 +1208,7 @@ static cudaError_t launch_tiles(PagedAttnArgs& a, int q_heads, cudaStream_t st) 
     static bool set[64] = {};
     cudaError_t e = pg_shared(paged_tile_kernel<T>, PT_SMEM, set);
     if (e == cudaSuccess) e = launch_chain(paged_tile_kernel<T>, dim3(grid), dim3(PT_THREADS), PT_SMEM, st, q, k, v, a);
-    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid, 16), dim3(PJ_THREADS), 0, st, a, 128);
+    if (e == cudaSuccess) e = launch_chain(paged_join_tiles_kernel<T>, dim3(grid, 4), dim3(PJ_THREADS), 0, st, a);
     return e;
 }
 
