@@ -166,7 +166,7 @@ __device__ __forceinline__ uint32_t pg_transpose(uint32_t w) {
 template <typename T, int NB>
 __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int COLS = 8 * NB, LD = 132;
-    constexpr int PL = NB <= 2 ? 2 : 1;               // planes of P: two where the products have room beside the bytes
+    constexpr int PL = 2;                             // planes of P: the products have room beside the bytes
     static_assert(COLS * LD * 4 <= PR_STAGES * PR_STAGE, "a warp's outputs fit its stages");
     extern __shared__ __align__(128) unsigned char pr_raw[];
     __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PR_WARPS];
@@ -532,6 +532,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     __shared__ float s_res[132];
 
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
+    if (tid < 96 && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(warp == 0 ? &tm_q : warp == 1 ? &tm_k : &tm_v) : "memory");
     pdl_launch();
     pdl_wait();
     pg_block_prefix<PT_THREADS>(a.sh, a.c.q_start, a.c.kv_len, s_prefix, s_sum);
@@ -1044,15 +1045,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Items that were cut: the block in whose run an item began has left word of it.  A warp a row, a lane four dims; the parts are added in the order of their keys.
+// Items that were cut: the block in whose run an item began has left word of it.  Blocks take rows in turn; the four warps of a block a quarter of the parts each, a lane
+// four dims; everything is added in a fixed order.
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int PJ_THREADS = 128;
 
 template <typename T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnArgs a, int part_rows) {
+    __shared__ float4 s_v[4][32];
+    __shared__ float2 s_ml[4];
     pdl_launch();
     pdl_wait();
-    const int lane = threadIdx.x & 31, block = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block = blockIdx.x;
     const int4 cut = *reinterpret_cast<const int4*>(&a.cuts[block]);
     const int parts = cut.x;
     if (parts == 0) return;
@@ -1061,38 +1065,52 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
     s.seq = pg_seq(a.sh, a.c.q_start, a.c.kv_len, s.b);
     const int live = min(1 << a.sh.tile_log, s.seq.q - (s.r << a.sh.tile_log)) << a.group_log;
     auto part = [&](int i, int row) { return a.part + ((size_t)(2 * (block + i) + (i == 0 ? cut.y : 0)) * part_rows + row) * PG_PART; };
-    for (int row = blockIdx.y * (PJ_THREADS / 32) + (threadIdx.x >> 5); row < live; row += gridDim.y * (PJ_THREADS / 32)) {
-        float M = -INFINITY;
-        bool nan = false;
-        for (int i = lane; i < parts; i += 32) { const float x = part(i, row)[0]; M = fmaxf(M, x); nan = nan || x != x; }
-        M = warp_max(M);
-        if (__any_sync(0xffffffffu, nan)) M = NAN;
-        const float Ms = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
+    const int each = (parts + 3) / 4, p0 = min(warp * each, parts), p1 = min(p0 + each, parts);
+    for (int row = blockIdx.y; row < live; row += gridDim.y) {
+        float M = -INFINITY, L = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < parts; i0 += 32) {
-            float w = 0.f, lw = 0.f;
-            if (i0 + lane < parts) {
-                const float2 ml = *reinterpret_cast<const float2*>(part(i0 + lane, row));
-                w = ml.x == -INFINITY ? 0.f : ml.x == Ms ? 1.f : pg_ex2(ml.x - Ms);
-                lw = ml.x == -INFINITY ? 0.f : ml.y * w;
-            }
-            L += warp_sum(lw);
-            const int n = min(32, parts - i0);
-            for (int i1 = 0; i1 < n; i1 += 8) {       // eight parts' loads under way
-                float4 x[8];
+        for (int i0 = p0; i0 < p1; i0 += 8) {        // eight parts' loads under way
+            float2 ml[8];
+            float4 x[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i1 + i < n) x[i] = *reinterpret_cast<const float4*>(part(i0 + i1 + i, row) + 4 + lane * 4);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float wi = __shfl_sync(0xffffffffu, w, (i1 + i) & 31);
-                    if (i1 + i < n && wi != 0.f) { v.x = fmaf(x[i].x, wi, v.x); v.y = fmaf(x[i].y, wi, v.y); v.z = fmaf(x[i].z, wi, v.z); v.w = fmaf(x[i].w, wi, v.w); }
+            for (int i = 0; i < 8; ++i)
+                if (i0 + i < p1) {
+                    ml[i] = *reinterpret_cast<const float2*>(part(i0 + i, row));
+                    x[i] = *reinterpret_cast<const float4*>(part(i0 + i, row) + 4 + lane * 4);
                 }
-            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i0 + i < p1 && ml[i].x != -INFINITY) {
+                    const float top = ml[i].x > M || ml[i].x != ml[i].x ? ml[i].x : M, f = M == top ? 1.f : pg_ex2(M - top), w = ml[i].x == top ? 1.f : pg_ex2(ml[i].x - top);
+                    M = top;
+                    L = L * f + ml[i].y * w;
+                    v.x = v.x * f + x[i].x * w; v.y = v.y * f + x[i].y * w; v.z = v.z * f + x[i].z * w; v.w = v.w * f + x[i].w * w;
+                }
         }
-        const float r = L > 0.f || L != L ? 1.f / L : 0.f;
-        *reinterpret_cast<uint2*>(pg_o_row(a, s, row) + lane * 8) = make_uint2(T::pack(v.x * r, v.y * r), T::pack(v.z * r, v.w * r));
+        s_v[warp][lane] = v;
+        if (lane == 0) s_ml[warp] = make_float2(M, L);
+        __syncthreads();
+        if (warp == 0) {
+            float top = -INFINITY;
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { top = fmaxf(top, s_ml[i].x); nan = nan || s_ml[i].x != s_ml[i].x; }
+            if (nan) top = NAN;
+            L = 0.f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float m = s_ml[i].x;
+                if (m == -INFINITY) continue;
+                const float w = m == top ? 1.f : pg_ex2(m - top);
+                const float4 x = s_v[i][lane];
+                L += s_ml[i].y * w;
+                v.x = fmaf(x.x, w, v.x); v.y = fmaf(x.y, w, v.y); v.z = fmaf(x.z, w, v.z); v.w = fmaf(x.w, w, v.w);
+            }
+            const float r = L > 0.f || L != L ? 1.f / L : 0.f;
+            *reinterpret_cast<uint2*>(pg_o_row(a, s, row) + lane * 8) = make_uint2(T::pack(v.x * r, v.y * r), T::pack(v.z * r, v.w * r));
+        }
+        __syncthreads();
     }
 }
 
@@ -1142,8 +1160,10 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_tiles_kernel(const Page
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// New tokens of a sequence up to which the products are the few-row kernel's: 32 rows with all q heads of a kv head.
-static bool pg_few(int max_new, int group) { return max_new * (long long)group <= 32; }
+// Up to 16 rows (new tokens times the q heads of a kv head) the few-row kernel has the products, beyond the tile kernel.  us a call, few-row / tile kernel: 8 sequences of up to
+// 5000 positions with 6 new tokens each, group 2 (12 rows) 31.4 / 37.2, fp16 31.6 / 38.5, 13 (26 rows, four column blocks) 48.7 / 39.1, fp16 48.6 / 40.3;
+// 16 sequences, 2 tokens, group 8 (16 rows) 24.8 / 28.4; one sequence of 300 positions and 13 tokens 24.9 / 22.7.
+static bool pg_few(int max_new, int group) { return max_new * (long long)group <= 16; }
 static int pg_log(int n) {
     int l = 0;
     while ((1 << l) < n) ++l;
@@ -1164,15 +1184,15 @@ static cudaError_t pg_shared(K* kernel, size_t bytes, bool (&set)[64]) {
 }
 
 template <typename T, int NB>
-static cudaError_t launch_rows(PagedAttnArgs& a, cudaStream_t st) {
+static cudaError_t launch_rows(PagedAttnArgs& a, int rows, cudaStream_t st) {
     a.sh.unit_log = PR_UNIT_LOG;
-    a.sh.tile_log = (NB == 1 ? 3 : NB == 2 ? 4 : 5) - a.group_log;
+    a.sh.tile_log = (NB == 1 ? 3 : 4) - a.group_log;
     a.least = 1;
     const int grid = 2 * tc_sm_count();
     static bool set[64] = {};
     cudaError_t e = pg_shared(paged_rows_kernel<T, NB>, PR_SMEM, set);
     if (e == cudaSuccess) e = launch_chain(paged_rows_kernel<T, NB>, dim3(grid), dim3(PR_THREADS), PR_SMEM, st, a);
-    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid, 2 * NB), dim3(PJ_THREADS), 0, st, a, 8 * NB);
+    if (e == cudaSuccess) e = launch_chain(paged_join_kernel<T>, dim3(grid, rows), dim3(PJ_THREADS), 0, st, a, 8 * NB);
     return e;
 }
 
@@ -1216,7 +1236,7 @@ template <typename T>
 static cudaError_t launch_attn(PagedAttnArgs& a, int max_new, int q_heads, cudaStream_t st) {
     if (!pg_few(max_new, 1 << a.group_log)) return launch_tiles<T>(a, q_heads, st);
     const int cols = max_new << a.group_log;
-    return cols <= 8 ? launch_rows<T, 1>(a, st) : cols <= 16 ? launch_rows<T, 2>(a, st) : launch_rows<T, 4>(a, st);
+    return cols <= 8 ? launch_rows<T, 1>(a, cols, st) : launch_rows<T, 2>(a, cols, st);
 }
 
 int paged_check(const char* who, const q3_paged* c) {
@@ -1257,13 +1277,13 @@ PagedView paged_view(const q3_paged* c) {
 using namespace q3;
 
 static int64_t pg_cut_bytes() { return ((int64_t)2 * tc_sm_count() * (int64_t)sizeof(PgCut) + 1023) / 1024 * 1024; }
-// a record a block, two partial results a block: 32 rows at most for each of two blocks an SM, or 128 for one
+// a record a block, two partial results a block: 16 rows at most for each of two blocks an SM, or 128 for one
 extern "C" int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads) {
     if (!c || q_heads < 1) return engine_fail(nullptr, Q3_ERR_INVALID, "q3_paged_attn_workspace: bad argument");
     const int sms = tc_sm_count();
     if (sms < 1) return engine_fail(nullptr, Q3_ERR_CUDA, "q3_paged_attn_workspace: no CUDA device");
     const int group = q_heads / (c->kv_heads < 1 ? 1 : c->kv_heads);
-    return pg_cut_bytes() + (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 32 : 128) * PG_PART * 4;
+    return pg_cut_bytes() + (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 16 : 128) * PG_PART * 4;
 }
 
 extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, void* stream) {
