@@ -10,7 +10,6 @@ documentation of the rule, not a fallback (`sample` fails without the CUDA libra
 from __future__ import annotations
 
 import contextlib
-import ctypes
 
 import torch
 
@@ -58,6 +57,8 @@ def sample_reference(logits: torch.Tensor, temperature: float, top_k: int, u: to
 
 
 _NO_SWITCH = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(device).cuda_stream without the Stream object
+_FILTERS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
 
 def sample_rows(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, u: torch.Tensor | None = None, generator: torch.Generator | None = None,
@@ -70,11 +71,11 @@ def sample_rows(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p
     Enqueues on the current stream of the logits' device and returns the int64 tokens [batch] (`out` when given) without synchronising; equal inputs draw equal words."""
     if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[0] < 1 or (logits.shape[1] != 1 and logits.stride(1) != 1):
         raise ValueError("sample_rows: logits must be a CUDA float32 tensor [batch, vocab] with contiguous words")
-    batch, vocab, dev = logits.shape[0], logits.shape[1], logits.device
-    ptrs, values = [], []
-    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    (batch, vocab), dev = logits.shape, logits.device
+    ptrs, values, size = [], [], (batch,)
+    for (name, dtype), x in zip(_FILTERS, (temperature, top_k, top_p, min_p)):
         if isinstance(x, torch.Tensor):
-            if x.dtype != dtype or x.shape != (batch,) or x.device != dev or not x.is_contiguous():
+            if x.dtype != dtype or x.shape != size or x.device != dev or not x.is_contiguous():
                 raise ValueError(f"sample_rows: {name} must be a number or a contiguous {dtype} tensor [{batch}] on {dev}")
             ptrs.append(x.data_ptr()), values.append(0)
         else:
@@ -91,7 +92,7 @@ def sample_rows(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p
     a = _cabi.SampleRowsArgs(logits.data_ptr(), logits.stride(0) if batch > 1 else vocab, *ptrs, u.data_ptr(), out.data_ptr(), batch, vocab, float(values[0]), int(values[1]),
                              float(values[2]), float(values[3]))
     with _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
-        rc = lib.q3_sample_rows(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+        rc = lib.q3_sample_rows(a, _raw_stream(dev.index))
     if rc:
         _cabi.check(lib, None, rc, "q3_sample_rows")
     return out
