@@ -10,11 +10,11 @@
 //
 // A CLUSTER of blocks a row.  Usually few words are kept:
 //   1. every thread finds the maximum of its words (and, where top-p or no filter at all needs the sum over the row, that sum, under its running maximum);
-//   2. the threads' maxima are binned over the cluster; the bins of the K largest maxima (K = top_k, or 512 for a nucleus) bound the row's K largest words from below.
-//      The few words at or above that bound go to the cluster's first block;
+//   2. the threads' maxima are binned over the cluster; the bins of the K largest maxima (K = top_k, or for a nucleus so many that about 850 words are expected there) bound the row's K largest words from below.  A nucleus
+//      is usually far smaller: the bound is where the maxima alone weigh enough; and no bound is lower than min_p's.  The few words at or above it go to the cluster's first block;
 //   3. which sorts them, cuts the sorted list by k, p and min_p, sorts what is kept by index and draws.
 // Where that is not enough (the nucleus is wider than the candidates, k > 512, many equal words) the element at the cut is searched with passes over the row (from
-// L2): eight brackets a pass, counts and weights of all of them, until a bracket's words fit the list; the draw then walks the row.
+// L2): bins of all words' counts and weights, then, while the words about the cut do not fit the list, eight brackets a pass; the draw then walks the row.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -27,7 +27,7 @@ namespace q3 {
 
 typedef unsigned long long u64;
 
-constexpr int SR_THREADS = 1024, SR_WARPS = 32, SR_MAX_CLUSTER = 16, SR_BINS = 2048, SR_LIST = 1024, SR_NUCLEUS = 512, SR_CUTS = 7;
+constexpr int SR_THREADS = 1024, SR_WARPS = 32, SR_MAX_CLUSTER = 16, SR_BINS = 512, SR_LIST = 1024, SR_NUCLEUS = 850, SR_CUTS = 7;
 constexpr float SR_FAR = 96.f;          // logits further than this many temperatures below the maximum weigh e^-96: no unit
 constexpr float SR_UNIT = 1099511627776.f;      // 2^40
 
@@ -60,6 +60,37 @@ __device__ __forceinline__ u64 sr_warp_sum(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += sr_shfl_xor(v, o);
     return v;
+}
+
+__device__ __forceinline__ u64 sr_pair(float lo, float hi) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 sr_unpair(u64 v) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+    return d;
+}
+__device__ __forceinline__ u64 sr_add2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 sr_mul2(u64 a, u64 b) {
+    u64 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float sr_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float sr_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 struct SampleRowsShared {
@@ -153,25 +184,32 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         v.z = i + 2 < i1 ? row[i + 2] : -INFINITY; v.w = i + 3 < i1 ? row[i + 3] : -INFINITY;
         return v;
     };
-    const int groups = (i1 - i0 + 127) / 128;
-    auto batches = [&](auto&& f) {                                     // f(first group, four groups' words); the next four are under way meanwhile
+    const int groups = (i1 - i0 + 127) / 128, whole = vec ? (i1 - i0) / 128 : 0;
+    auto batches = [&](auto&& f) {                                     // f(four groups' words); the next four are under way meanwhile
         float4 v[2][4];
         auto load = [&](int j, float4 (&d)[4]) {
+            if (j + 4 <= whole) {                                      // (no guards)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) d[q] = fetch(j + q, lane);
+                for (int q = 0; q < 4; ++q) d[q] = *reinterpret_cast<const float4*>(row + i0 + 128 * (j + q) + 4 * lane);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) d[q] = fetch(j + q, lane);
+            }
         };
         if (groups > 0) load(0, v[0]);
         for (int j = 0; j < groups; j += 8) {
             if (j + 4 < groups) load(j + 4, v[1]);
-            f(j, v[0]);
+            f(v[0]);
             if (j + 8 < groups) load(j + 8, v[0]);
-            if (j + 4 < groups) f(j + 4, v[1]);
+            if (j + 4 < groups) f(v[1]);
         }
     };
     auto each = [&](auto&& f) {                                        // f(index, word) over this thread's words, in ascending order (paths that few rows take)
+        float4 next = groups > 0 ? fetch(0, lane) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
         for (int j = 0; j < groups; ++j) {
-            const float4 v = fetch(j, lane);
+            const float4 v = next;
+            if (j + 1 < groups) next = fetch(j + 1, lane);
             const int i = i0 + 128 * j + 4 * lane;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q)
@@ -182,21 +220,35 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
     // ---- 1. maxima and, where needed, sums ----
     float mine = -INFINITY, wsum = 0.f;
     bool odd = false;                                                  // a word is no number
-    batches([&](int, const float4 (&v)[4]) {
+    const float c_t = inv_t * 1.4426950408889634f;
+    const u64 c2 = sr_pair(c_t, c_t);
+    u64 sum2 = 0ull;                                                   // (two words an instruction)
+    batches([&](const float4 (&v)[4]) {
         float top = -INFINITY;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            top = fmaxf(top, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)));
+            top = sr_max3(sr_max3(top, v[q].x, v[q].y), v[q].z, v[q].w);
             odd = odd || v[q].x != v[q].x || v[q].y != v[q].y || v[q].z != v[q].z || v[q].w != v[q].w;
         }
-        if (summed) {
-            if (top > mine) { if (mine > -INFINITY) wsum *= __expf(fmaxf(mine - top, -FLT_MAX) * inv_t); mine = top; }
+        if (!summed) { mine = fmaxf(mine, top); return; }
+        if (top > mine) {
+            if (mine > -INFINITY) { const float f = sr_ex2(fmaxf(mine - top, -FLT_MAX) * c_t); sum2 = sr_mul2(sum2, sr_pair(f, f)); }
+            mine = top;
+        }
+        if (mine == -INFINITY) return;
+        const u64 less = sr_pair(-mine, -mine);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) wsum += (weight(v[q].x, mine) + weight(v[q].y, mine)) + (weight(v[q].z, mine) + weight(v[q].w, mine));
-        } else {
-            mine = fmaxf(mine, top);
+        for (int q = 0; q < 4; ++q) {
+            // (a masked word: -inf times the factor is -inf, of weight 0; only a factor of 0 needs a look)
+            float2 x = sr_unpair(sr_mul2(sr_add2(sr_pair(v[q].x, v[q].y), less), c2)), y = sr_unpair(sr_mul2(sr_add2(sr_pair(v[q].z, v[q].w), less), c2));
+            if (c_t == 0.f) {
+                x.x = v[q].x < -FLT_MAX ? -INFINITY : 0.f; x.y = v[q].y < -FLT_MAX ? -INFINITY : 0.f;
+                y.x = v[q].z < -FLT_MAX ? -INFINITY : 0.f; y.y = v[q].w < -FLT_MAX ? -INFINITY : 0.f;
+            }
+            sum2 = sr_add2(sum2, sr_add2(sr_pair(sr_ex2(x.x), sr_ex2(x.y)), sr_pair(sr_ex2(y.x), sr_ex2(y.y))));
         }
     });
+    if (summed) { const float2 s = sr_unpair(sum2); wsum = s.x + s.y; }
     for (int b = tid; b < SR_BINS; b += SR_THREADS) sh.hist[b] = 0u;
     {
         const float bv = sr_warp_max(mine), lo = -sr_warp_max(mine >= -FLT_MAX ? -mine : -INFINITY);
@@ -263,20 +315,31 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         if (tid == 0) sh.sel = SR_BINS - 1;
         cluster.sync();
         {
-            // thread t: bins 2 t and 2 t + 1 over the cluster; the bin in which the running count reaches K
-            unsigned c0 = 0u, c1 = 0u;
-            for (int r = 0; r < C; ++r) {
-                const uint2 h = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&sh, r)->hist + 2 * tid);
-                c0 += h.x; c1 += h.y;
+            // thread t: bin t over the cluster.  The bound is the bin in which the count of the threads' maxima reaches K, or, for a nucleus, before that the one with which
+            // these maxima alone weigh enough (each taken at its bin's far end).  (512 bins: every block reads every other's, 2048 cost one row 2 us more)
+            unsigned c = 0u;
+            if (tid < SR_BINS)
+#pragma unroll
+                for (int r = 0; r < SR_MAX_CLUSTER; ++r)
+                    if (r < C) c += cluster.map_shared_rank(&sh, r)->hist[tid];
+            const unsigned need = by_k ? (unsigned)k : (unsigned)a.nucleus;
+            const u64 incl = sr_scan(sh, (u64)c), before = incl - c;
+            if (before < need && incl >= need) atomicMin(&sh.sel, (unsigned)tid);
+            if (by_p && !by_k) {
+                const u64 mass = (u64)c * sr_units(sr_ex2(-(float)(tid + 1) * (c_t / scale))), upto = sr_scan(sh, mass);
+                const double reach = (double)p * (double)row_sum * 1.00001;
+                if ((double)(upto - mass) < reach && (double)upto >= reach) atomicMin(&sh.sel, (unsigned)tid);
             }
-            const unsigned need = by_k ? (unsigned)min(k, a.vocab) : (unsigned)a.nucleus;
-            const unsigned incl = (unsigned)sr_scan(sh, (u64)(c0 + c1)), before = incl - c0 - c1;
-            if (before < need && incl >= need) sh.sel = 2 * tid + (before + c0 < need ? 1 : 0);
             __syncthreads();
         }
         int last = (int)sh.sel;
         if (clipped) last = min(last, SR_BINS - 2);
-        const bool all = last == SR_BINS - 1 || (clipped && last == SR_BINS - 2);     // every word with a weight is a candidate
+        // words below min_p are not kept, whatever the others are (but where top-p asks for the k largest's sum): its bin bounds the candidates, too
+        int floor_bin = SR_BINS;
+        if (min_p > 0.f && !(by_k && by_p)) floor_bin = (int)fminf(-__logf(min_p) * T * scale * 1.0001f, (float)SR_BINS) + 1;
+        const bool floored = floor_bin <= last;
+        last = min(last, floor_bin);
+        const bool all = floored || last == SR_BINS - 1 || (clipped && last == SR_BINS - 2);     // every word that may be kept is a candidate
         SampleRowsShared* const first = cluster.map_shared_rank(&sh, 0);
         auto take = [&](int i, float v) {
             if (i < i1 && v >= -FLT_MAX && bin(v) <= last) {
@@ -348,9 +411,78 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
         // ---- the cut by passes over the row ----
         // The smallest element that is kept when elements are taken in descending order until their count (of_count) or weight reaches `need`.
         auto search = [&](bool of_count, double need, u64 floor) -> u64 {
-            u64 lo = floor, hi = ((u64)sr_key(vmax) + 1) << 32, hi_w = 0ull;      // everything at or above hi is kept and short of `need`
-            unsigned hi_c = 0u, lo_c = 0xffffffffu;
             auto reached = [&](unsigned c, u64 w) { return of_count ? (double)c >= need : (double)w >= need; };
+            // Where the cut lies to within a bin: counts of all words, and their weights in 2^-31 of a bound of the sum.  Such sums are off by half a unit a word, so the bins
+            // between which the cut lies are those with which it may be reached and with which it must be.
+            const double unit = 2147483648.0 / ((double)row_sum > 0. ? (double)row_sum * 1.001 : 1099511627776.0 * vocab) * 1099511627776.0;
+            unsigned* const mass = reinterpret_cast<unsigned*>(sh.weight);
+            __syncthreads();
+            for (int b = tid; b < SR_BINS; b += SR_THREADS) { sh.hist[b] = 0u; mass[b] = 0u; }
+            if (tid == 0) { sh.sel = SR_BINS - 1; sh.n = SR_BINS - 1; }
+            __syncthreads();
+            {
+                unsigned far_c = 0u, far_m = 0u;                  // the last bin's, which holds most words, stay with the thread
+                each([&](int i, float v) {
+                    if (v >= -FLT_MAX && sr_element(v, i) >= floor) {
+                        const int b = bin(v);
+                        const unsigned m = (unsigned)(weight(v, vmax) * (float)unit + 0.5f);
+                        if (b == SR_BINS - 1) { ++far_c; far_m += m; }
+                        else { atomicAdd(&sh.hist[b], 1u); if (m) atomicAdd(&mass[b], m); }
+                    }
+                });
+                far_c = __reduce_add_sync(0xffffffffu, far_c); far_m = __reduce_add_sync(0xffffffffu, far_m);
+                if (lane == 0) { atomicAdd(&sh.hist[SR_BINS - 1], far_c); atomicAdd(&mass[SR_BINS - 1], far_m); }
+            }
+            cluster.sync();
+            {
+                unsigned c = 0u;
+                u64 m = 0ull;
+                if (tid < SR_BINS)
+                    for (int r = 0; r < C; ++r) {
+                        SampleRowsShared* peer = cluster.map_shared_rank(&sh, r);
+                        c += peer->hist[tid]; m += reinterpret_cast<unsigned*>(peer->weight)[tid];
+                    }
+                const u64 cc = sr_scan(sh, c), mm = sr_scan(sh, m);
+                const double want = of_count ? need : need * (unit / 1099511627776.0), have = of_count ? (double)cc : (double)mm, err = of_count ? 0. : 0.51 * (double)cc + 1. + 1e-6 * want;
+                if (tid < SR_BINS && have + err >= want) atomicMin(&sh.sel, (unsigned)tid);
+                if (tid < SR_BINS && have - err >= want) atomicMin(&sh.n, (unsigned)tid);
+            }
+            __syncthreads();
+            const int b1 = (int)sh.sel, b2 = (int)sh.n;
+            // the smallest element whose word's bin is at most b
+            auto bound = [&](int b) -> u64 {
+                unsigned key = 0u;                                // the largest key of a bin beyond b: keys ascend, bins descend
+                for (int bit = 31; bit >= 0; --bit) {
+                    const unsigned trial = key | (1u << bit);
+                    const float v = sr_value(trial);
+                    if (trial <= sr_key(vmax) && (v != v || v < -FLT_MAX || bin(v) > b)) key = trial;
+                }
+                return (u64)(key + 1u) << 32;
+            };
+            u64 lo = b2 >= SR_BINS - 1 ? floor : max(floor, bound(b2)), hi = b1 == 0 ? ((u64)sr_key(vmax) + 1) << 32 : max(lo, bound(b1 - 1)), hi_w = 0ull;      // everything at or above hi is kept
+            unsigned hi_c = 0u, lo_c = 0xffffffffu;
+            {
+                unsigned c = 0u;
+                u64 w = 0ull;
+                each([&](int i, float v) {
+                    if (v >= -FLT_MAX && sr_element(v, i) >= hi) { ++c; w += sr_units(weight(v, vmax)); }
+                });
+                c = __reduce_add_sync(0xffffffffu, c); w = sr_warp_sum(w);
+                if (lane == 0) { sh.wcutc[warp][0] = c; sh.wcutw[warp][0] = w; }
+                __syncthreads();
+                if (warp == 0) {
+                    c = __reduce_add_sync(0xffffffffu, sh.wcutc[lane][0]); w = sr_warp_sum(sh.wcutw[lane][0]);
+                    if (lane < C) {
+                        SampleRowsShared* peer = cluster.map_shared_rank(&sh, lane);
+                        peer->cutc[rank][0] = c; peer->cutw[rank][0] = w;
+                    }
+                }
+                cluster.sync();
+                for (int r = 0; r < C; ++r) { hi_c += sh.cutc[r][0]; hi_w += sh.cutw[r][0]; }
+                cluster.sync();                                   // every block has read
+                // (the count of a nucleus' bins and its exact sum may differ about a border: the words at or above hi reach it by themselves)
+                if (hi_c > 0u && reached(hi_c, hi_w)) { hi = ((u64)sr_key(vmax) + 1) << 32; hi_c = 0u; hi_w = 0ull; }
+            }
             for (;;) {
                 const u64 step = (hi - lo) / (SR_CUTS + 1);
                 if (lo_c != 0xffffffffu && (lo_c - hi_c <= SR_LIST || step == 0)) break;
@@ -393,12 +525,16 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
                     u64 wj = hi_w;
                     for (int r = 0; r < C; ++r) { cj += sh.cutc[r][j]; wj += sh.cutw[r][j]; }
                     if (new_lc == 0u) {
-                        if (reached(cj, wj) || j == 0) { new_lo = cut[j]; new_lc = cj; if (j == 0 && !reached(cj, wj)) { new_lc = 0xfffffffeu; } }
+                        if (reached(cj, wj) || j == 0) { new_lo = cut[j]; new_lc = cj; if (j == 0 && !reached(cj, wj)) { new_lc = 0xfffffffeu; new_hc = cj; new_hw = wj; } }
                         else { new_hi = cut[j]; new_hc = cj; new_hw = wj; }
                     }
                 }
                 cluster.sync();                                   // every block has read
-                if (new_lc == 0xfffffffeu) return floor;          // all words together fall short: all are kept
+                if (new_lc == 0xfffffffeu) {
+                    if (lo == floor) return floor;                // all words together fall short: all are kept
+                    hi = lo; hi_c = new_hc; hi_w = new_hw; lo = floor; lo_c = 0xffffffffu;
+                    continue;
+                }
                 lo = new_lo; hi = new_hi; hi_w = new_hw; hi_c = new_hc; lo_c = new_lc;
             }
             // the bracket's words, sorted by the first block
@@ -496,12 +632,15 @@ extern "C" int q3_sample_rows(const q3_sample_rows_args* p, void* stream) {
                             reinterpret_cast<uintptr_t>(p->top_ks) | reinterpret_cast<uintptr_t>(p->top_ps) | reinterpret_cast<uintptr_t>(p->min_ps);
     if ((words & 3) || (reinterpret_cast<uintptr_t>(p->out_tokens) & 7)) return bad("logits and parameters must be 4-byte aligned, out_tokens 8-byte aligned");
     SampleRowsArgs a{};
-    a.logits = p->logits; a.row_stride = p->row_stride; a.vocab = p->vocab; a.nucleus = SR_NUCLEUS;
+    a.logits = p->logits; a.row_stride = p->row_stride; a.vocab = p->vocab;
     a.temperature = p->temperatures; a.top_p = p->top_ps; a.min_p = p->min_ps; a.top_k = p->top_ks;
     a.temperature1 = p->temperature; a.top_p1 = p->top_p; a.min_p1 = p->min_p; a.top_k1 = p->top_k;
     a.uniform = p->uniform; a.out = reinterpret_cast<long long*>(p->out_tokens);
     int cluster = p->batch <= 4 ? 16 : p->batch <= 14 ? 8 : p->batch <= 36 ? 4 : p->batch <= 74 ? 2 : 1;
     while (cluster > 1 && p->vocab < cluster * SR_THREADS) cluster /= 2;
+    // N threads of which k hold words beyond a bound hold -N ln(1 - k/N) of them, if words are spread evenly: SR_NUCLEUS leaves the list of SR_LIST room for a bin more
+    // (512 maxima whatever N: 27 mixed rows up to 210 us, where one has a nucleus of 500 words or more; now 43 at most over 200 draws, 25 in the middle)
+    a.nucleus = (int)(cluster * SR_THREADS * (1. - exp(-(double)SR_NUCLEUS / (cluster * SR_THREADS))));
     cudaError_t e = cluster > 8 ? cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : cudaSuccess;
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
