@@ -1,8 +1,10 @@
 // The new tokens' q, k and v rows: head norm, rotary embedding, k and v into the pages of their sequences.
 //
-// A warp takes eight head rows of one token, a lane four neighbouring dims of each: all eight are requested before the first is used, the squares of a head
-// meet in a warp's sum and RoPE's pairs in a shuffle (half layout: the lane rotary / 8 further; interleaved: the lane itself).  Bound by bytes for many tokens, by
-// latency for few: one launch, three dependent loads (descriptors, page, rows and table meanwhile).
+// A warp takes four head rows of one token, two at a time: sixteen lanes a row, each with four dims and the four that they are rotated with (half layout; what is
+// not rotated is dealt out in eights).  So a rotation stays within its lane and the squares of a head meet in four shuffles.  All rows are requested before the first is used.
+// Bound by bytes for many tokens, by latency for few: one launch, three dependent loads (descriptors, page, table; the rows meanwhile).  2048 tokens of 16 + 8 + 8 fp32
+// heads: 50 MB in 14.4 us, 3.5 TB/s of the 6.5 that a copy reaches, some 4 us of it the launch and the first loads' chain (a lane with four neighbouring dims of a whole
+// row and its partner by shuffles: 20.1; sixteen lanes a row, 8 rows a warp in blocks of 256: 17.1, of 128: 14.9; 2 rows a warp: 17.0).
 #include <cuda_fp16.h>
 
 #include "q3_engine.h"
@@ -10,7 +12,7 @@
 
 namespace q3 {
 
-constexpr int RP_THREADS = 256, RP_ROWS = 8;          // head rows a warp takes
+constexpr int RP_THREADS = 128, RP_ROWS = 4;          // head rows a warp takes
 
 struct PagedRopeArgs {
     PagedView c;
@@ -49,20 +51,23 @@ template <int TYPE, bool BF>
 __global__ void __launch_bounds__(RP_THREADS) paged_rope_kernel(const PagedRopeArgs a) {
     pdl_launch();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warps = (a.q_heads + a.kv_rows + RP_ROWS - 1) / RP_ROWS;
+    const int lane = threadIdx.x & 31, part = lane & 15, second = lane >> 4, rows = a.q_heads + a.kv_rows, kv = a.sh.heads, warps = (rows + RP_ROWS - 1) / RP_ROWS;
     const long long w = (long long)blockIdx.x * (RP_THREADS / 32) + uniform_warp();
     const long long t = w / warps;
     if (t >= a.sh.n_tokens) return;
-    const int r0 = (int)(w - t * warps) * RP_ROWS;
-    // the rows: q heads, then k heads, then v heads
-    const int rows = a.q_heads + a.kv_rows, kv = a.sh.heads;
-    float4 x[RP_ROWS];
+    const int r0 = (int)(w - t * warps) * RP_ROWS + second;
+    // this lane's dims: d0 .. d0 + 3 and d1 .. d1 + 3
+    const int half = a.rotary / 2, d = part * 4;
+    const bool turned = a.interleaved || d < half;
+    const int d0 = turned ? d : a.rotary + (d - half) * 2, d1 = a.interleaved ? d + HEAD_DIM / 2 : turned ? d + half : d0 + 4;
+    constexpr int SIZE = TYPE == Q3_TYPE_FP32 ? 4 : 2;
+    float4 x[RP_ROWS / 2][2];
 #pragma unroll
-    for (int i = 0; i < RP_ROWS; ++i) {
-        const int r = min(r0 + i, rows - 1);
+    for (int i = 0; i < RP_ROWS / 2; ++i) {
+        const int r = min(r0 + 2 * i, rows - 1);      // the rows: q heads, then k heads, then v heads
         const unsigned char* src = r < a.q_heads ? a.q + t * a.q_token + r * a.q_head : r < a.q_heads + kv ? a.k + t * a.k_token + (r - a.q_heads) * a.k_head
                                                                                       : a.v + t * a.v_token + (r - a.q_heads - kv) * a.v_head;
-        x[i] = rp_load<TYPE>(src + lane * (TYPE == Q3_TYPE_FP32 ? 16 : 8));
+        x[i][0] = rp_load<TYPE>(src + d0 * SIZE); x[i][1] = rp_load<TYPE>(src + d1 * SIZE);
     }
     // the token's sequence: as many as end at or before it come before
     int b = 0;
@@ -75,54 +80,70 @@ __global__ void __launch_bounds__(RP_THREADS) paged_rope_kernel(const PagedRopeA
     const int page = place >= 0 && a.kv_rows ? pg_page(a.c, b, place) : -1;
     const int pos = a.positions ? a.positions[t] : place;
     const long long slot = page < 0 ? -1 : pg_offset(a.c, page, place & ((1 << a.c.page_log) - 1), 0);
-    // this lane's cosines and sines; what is not rotated is multiplied by one
-    const int half = a.rotary / 2, d = lane * 4;
-    const bool turned = d < a.rotary;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
-    if (turned) {
-        const bool known = pos >= 0 && pos < a.rope_positions;
-        const float* tab = a.rope + (size_t)(known ? pos : 0) * a.rotary;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int f = a.interleaved ? (d + i) >> 1 : d < half ? d + i : d + i - half;
-            c[i] = known ? tab[f] : NAN;
-            sn[i] = known ? tab[half + f] : NAN;
+    // this lane's cosines and sines: of d0 .. d0 + 3 and their partners d1 .., or of two pairs in each; what is not rotated is multiplied by one
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pos < 0 || pos >= a.rope_positions) {
+        if (a.interleaved ? d0 < a.rotary : turned) c.x = c.y = c.z = c.w = sn.x = sn.y = sn.z = sn.w = NAN;
+        if (a.interleaved && d1 >= a.rotary) { c.z = c.w = 1.f; sn.z = sn.w = 0.f; }
+    } else {
+        const float* const tab = a.rope + (size_t)pos * a.rotary;
+        if (a.interleaved) {
+            if (d0 < a.rotary) { c.x = tab[d0 / 2]; c.y = tab[d0 / 2 + 1]; sn.x = tab[half + d0 / 2]; sn.y = tab[half + d0 / 2 + 1]; }
+            if (d1 < a.rotary) { c.z = tab[d1 / 2]; c.w = tab[d1 / 2 + 1]; sn.z = tab[half + d1 / 2]; sn.w = tab[half + d1 / 2 + 1]; }
+        } else if (turned) {
+            if ((reinterpret_cast<uintptr_t>(a.rope) & 15) == 0) {
+                c = *reinterpret_cast<const float4*>(tab + d); sn = *reinterpret_cast<const float4*>(tab + half + d);
+            } else {
+                c = make_float4(tab[d], tab[d + 1], tab[d + 2], tab[d + 3]);
+                sn = make_float4(tab[half + d], tab[half + d + 1], tab[half + d + 2], tab[half + d + 3]);
+            }
         }
     }
-    const bool low = d < half;
-    const int other = turned ? (low ? lane + half / 4 : lane - half / 4) : lane;
-    const float q_g[4] = {a.q_gain ? bf_to_f(a.q_gain[d]) : 1.f, a.q_gain ? bf_to_f(a.q_gain[d + 1]) : 1.f, a.q_gain ? bf_to_f(a.q_gain[d + 2]) : 1.f, a.q_gain ? bf_to_f(a.q_gain[d + 3]) : 1.f};
-    const float k_g[4] = {a.k_gain ? bf_to_f(a.k_gain[d]) : 1.f, a.k_gain ? bf_to_f(a.k_gain[d + 1]) : 1.f, a.k_gain ? bf_to_f(a.k_gain[d + 2]) : 1.f, a.k_gain ? bf_to_f(a.k_gain[d + 3]) : 1.f};
+    auto gains = [&](const bf16_raw* g, int at) {     // four of them, packed
+        return g ? make_uint2(g[at] | (unsigned)g[at + 1] << 16, g[at + 2] | (unsigned)g[at + 3] << 16) : make_uint2(0x3f803f80u, 0x3f803f80u);
+    };
+    const uint2 gq0 = gains(a.q_gain, d0), gq1 = gains(a.q_gain, d1), gk0 = gains(a.k_gain, d0), gk1 = gains(a.k_gain, d1);
 #pragma unroll
-    for (int i = 0; i < RP_ROWS; ++i) {
-        const int r = r0 + i;
-        if (r >= rows) break;
-        float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        if (r < a.q_heads + kv) {
-            const bool is_q = r < a.q_heads;
-            if (is_q ? a.q_gain != nullptr : a.k_gain != nullptr) {
-                const float n = rsqrtf(warp_sum(fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3])))) / (float)HEAD_DIM + a.eps);
+    for (int i = 0; i < RP_ROWS / 2; ++i) {
+        const int r = r0 + 2 * i;
+        float4 y = x[i][0], z = x[i][1];
+        const bool is_q = r < a.q_heads;
+        if (__any_sync(0xffffffffu, r < a.q_heads + kv)) {
+            float n = fmaf(y.x, y.x, fmaf(y.y, y.y, fmaf(y.z, y.z, y.w * y.w))) + fmaf(z.x, z.x, fmaf(z.y, z.y, fmaf(z.z, z.z, z.w * z.w)));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = v[j] * n * (is_q ? q_g[j] : k_g[j]);
-            }
-            if (a.rotary) {
-                float p[4];
-                if (a.interleaved) { p[0] = -v[1]; p[1] = v[0]; p[2] = -v[3]; p[3] = v[2]; }
-                else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { p[j] = __shfl_sync(0xffffffffu, v[j], other); if (low) p[j] = -p[j]; }
+            for (int o = 8; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+            if (r < a.q_heads + kv) {
+                if (is_q ? a.q_gain != nullptr : a.k_gain != nullptr) {
+                    const uint2 g0 = is_q ? gq0 : gk0, g1 = is_q ? gq1 : gk1;
+                    n = rsqrtf(n / (float)HEAD_DIM + a.eps);
+                    y.x = y.x * n * bf_lo(g0.x); y.y = y.y * n * bf_hi(g0.x); y.z = y.z * n * bf_lo(g0.y); y.w = y.w * n * bf_hi(g0.y);
+                    z.x = z.x * n * bf_lo(g1.x); z.y = z.y * n * bf_hi(g1.x); z.z = z.z * n * bf_lo(g1.y); z.w = z.w * n * bf_hi(g1.y);
                 }
-                if (turned)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = fmaf(p[j], sn[j], v[j] * c[j]);
+                const float4 p = y, q = z;
+                if (a.interleaved) {
+                    if (d0 < a.rotary) {
+                        y.x = fmaf(-p.y, sn.x, p.x * c.x); y.y = fmaf(p.x, sn.x, p.y * c.x);
+                        y.z = fmaf(-p.w, sn.y, p.z * c.y); y.w = fmaf(p.z, sn.y, p.w * c.y);
+                    }
+                    if (d1 < a.rotary) {
+                        z.x = fmaf(-q.y, sn.z, q.x * c.z); z.y = fmaf(q.x, sn.z, q.y * c.z);
+                        z.z = fmaf(-q.w, sn.w, q.z * c.w); z.w = fmaf(q.z, sn.w, q.w * c.w);
+                    }
+                } else if (turned) {
+                    y.x = fmaf(-q.x, sn.x, p.x * c.x); y.y = fmaf(-q.y, sn.y, p.y * c.y); y.z = fmaf(-q.z, sn.z, p.z * c.z); y.w = fmaf(-q.w, sn.w, p.w * c.w);
+                    z.x = fmaf(p.x, sn.x, q.x * c.x); z.y = fmaf(p.y, sn.y, q.y * c.y); z.z = fmaf(p.z, sn.z, q.z * c.z); z.w = fmaf(p.w, sn.w, q.w * c.w);
+                }
             }
         }
-        const uint2 u = rp_pack<BF>(make_float4(v[0], v[1], v[2], v[3]));
-        if (r < a.q_heads) *reinterpret_cast<uint2*>(a.out + t * a.o_token + r * a.o_head + lane * 8) = u;
+        if (r >= rows) continue;
+        unsigned char* to;
+        if (is_q) to = a.out + t * a.o_token + r * a.o_head;
         else if (slot >= 0) {
             const int h = r - a.q_heads;
-            *reinterpret_cast<uint2*>((h < kv ? a.c.k + h * a.c.head_bytes : a.c.v + (h - kv) * a.c.head_bytes) + slot + lane * 8) = u;
-        }
+            to = (h < kv ? a.c.k + h * a.c.head_bytes : a.c.v + (h - kv) * a.c.head_bytes) + slot;
+        } else continue;
+        *reinterpret_cast<uint2*>(to + 2 * d0) = rp_pack<BF>(y);
+        *reinterpret_cast<uint2*>(to + 2 * d1) = rp_pack<BF>(z);
     }
 }
 
