@@ -397,9 +397,10 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
 //
 // bf16: P has fp32's exponents, so that m need not be the maximum: the largest score of the segment's first tile (0 where a row sees none of it) serves all its
 // tiles.  Nothing is rescaled, no other tile is searched for its maximum, one O serves all groups, and there is room for three S.  A row that leaves fp32's range (scores 88 above the first tile's) is not finite at the end, one that has vanished (no weight
-// above 2^-100 though it sees keys) is seen by its sum: both are done again row by row.  P is truncated to bf16, and its sum is that of the truncated values, which takes
-// the truncation's mean out of the quotient: what is left of it is as large as of rounding (a conversion would be the special-function pipe's, like the exponentials).
+// above 2^-100 though it sees keys) is seen by its sum: both are done again row by row.
 // fp16: P must not leave [2^-24, 2^16), so m follows a group's maximum, and its O is rescaled when a score exceeds m by 2^8; two S and two O.
+// P is rounded to the pages' type and its sum is that of the rounded values: where few keys hold a row's weight their roundings leave the quotient.  2048 tokens
+// behind 8192: 2.3e-3 off, 1.7e-3 of it the output's own rounding (P truncated, as fast: 2.4e-3, and 2.6e-3 with short sequences).
 //
 // A wait that gives up lets every later one give up at once (those in which the softmax warps meet are waits like the others); the block then drains what is under way and
 // leaves NaN in all rows of its run.
@@ -822,13 +823,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                         for (int j = 0; j < 16; ++j) {
                             const float2 x2 = pt_unpair(pt_fma2(pt_pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2, m2));
                             const float e0 = pg_ex2(x2.x), e1 = pg_ex2(x2.y);
-                            if constexpr (ONE) {
-                                pk[j] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
-                                sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(__uint_as_float(__float_as_uint(e0) & 0xffff0000u), __uint_as_float(__float_as_uint(e1) & 0xffff0000u)));
-                            } else {
-                                pk[j] = T::pack(e0, e1);
-                                sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(e0, e1));
-                            }
+                            pk[j] = T::pack(e0, e1);
+                            const float2 y = T::unpack(pk[j]);
+                            sum2[j & 1] = pt_add2(sum2[j & 1], pt_pair(y.x, y.y));
                         }
                         pt_st16(ts + (uint32_t)(h * 16), pk);                // (over scores that have been read)
                     };
