@@ -762,10 +762,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 auto hide = [&](uint32_t (&r)[32], int h) {                  // what the row does not see of the tile's quarter h
                     const int most = last - tile0 - h * 32;
-                    const unsigned gone = ~(pages >> (h * 2));
+                    const unsigned there = (pages >> (h * 2)) & 3u;
+                    const unsigned sees = (most >= 31 ? 0xffffffffu : most < 0 ? 0u : (2u << most) - 1u) & ((there & 1u ? 0xffffu : 0u) | (there & 2u ? 0xffff0000u : 0u));
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (j > most || ((gone >> (j >> 4)) & 1u)) r[j] = 0xff800000u;            // -inf
+                        if (!((sees >> j) & 1u)) r[j] = 0xff800000u;            // -inf
                 };
                 if (live && (!ONE || t == 0)) {
                     float x[2] = {-INFINITY, -INFINITY};
@@ -914,7 +915,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if (!whole && row < d.rows) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(mx, sum);
                 unsigned char* const o_row = a.out + (long long)(d.q_row + (row >> a.group_log)) * a.o_token + (long long)((d.h << a.group_log) + (row & ((1 << a.group_log) - 1))) * a.o_head;
                 uint64_t odd = 0ull;                 // 0, or NaN once an output is not finite
-                if (live) {
+                if (ONE && live && whole && n > 0) {         // O is free for the next segment's before its rows are stored
+                    uint32_t pk[64];
+                    const uint64_t r2 = pt_pair(r, r);
+#pragma unroll
+                    for (int e = 0; e < HEAD_DIM; e += 32) {
+                        uint32_t v[32];
+                        tc_ld32(v, trow + 384u + (uint32_t)e);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t o = pt_pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            odd = pt_fma2(o, 0ull, odd);
+                            const float2 x = pt_unpair(pt_fma2(o, r2, 0x8000000080000000ull));
+                            pk[e / 2 + j] = T::pack(x.x, x.y);
+                        }
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) pt_arrive(&o_free);
+                    if (row < d.rows)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) *reinterpret_cast<uint4*>(o_row + j * 16) = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+                } else if (live) {
 #pragma unroll 1
                     for (int e = 0; e < HEAD_DIM; e += 32) {
                         uint64_t o[16];
