@@ -89,7 +89,7 @@ def sample_rows(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p
     elif out.dtype != torch.int64 or out.shape != (batch,) or out.device != dev or not out.is_contiguous():
         raise ValueError(f"sample_rows: out must be a contiguous int64 tensor [{batch}] on {dev}")
     lib = _cabi.load()
-    a = _cabi.SampleRowsArgs(logits.data_ptr(), logits.stride(0) if batch > 1 else vocab, *ptrs, u.data_ptr(), out.data_ptr(), batch, vocab, float(values[0]), int(values[1]),
+    a = _cabi.SampleRowsArgs(logits.data_ptr(), logits.stride(0) if batch > 1 else vocab, *ptrs, u.data_ptr(), out.data_ptr(), batch, vocab, float(values[0]), min(int(values[1]), 0x7fffffff),
                              float(values[2]), float(values[3]))
     with _NO_SWITCH if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
         rc = lib.q3_sample_rows(a, _raw_stream(dev.index))

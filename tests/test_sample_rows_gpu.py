@@ -234,3 +234,20 @@ def test_bad_arguments_are_refused_before_the_device_is_touched():
         assert lib.q3_last_error(None).startswith(b"q3_sample_rows: ")
     assert lib.q3_sample_rows(None, None) == _cabi.ERR_INVALID
     assert ctypes.sizeof(_cabi.SampleRowsArgs) == 8 * 8 + 6 * 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1e-39, 1e-37, 1e-20, 1e30, 1e37, float("inf")])
+@pytest.mark.parametrize("setting", [(0, 1.0, 0.0), (0, 0.9, 0.0), (50, 1.0, 0.0), (0, 1.0, 0.1), (100, 0.9, 0.05)])
+def test_extreme_temperatures_and_logits(t, setting):
+    from qwen3mk import sampling
+
+    g = torch.Generator().manual_seed(6)
+    logits = torch.randn(6, 5000, generator=g) * 4
+    logits[1] *= 7e37 / logits[1].abs().max()
+    logits[2, ::2], logits[2, 1::2] = 3e38, -3e38
+    logits[3] = -7.0
+    logits[4, 100:] = float("-inf")
+    logits = logits.cuda()
+    u = torch.rand(6, generator=g).cuda()
+    verify(logits, sampling.sample_rows(logits, t, *setting, u=u), u, t, *setting)
