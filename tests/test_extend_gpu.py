@@ -213,3 +213,26 @@ def test_null_engines_are_refused():
 
     lib = _cabi.load()
     assert lib.q3_extend(None, None, None) == _cabi.ERR_INVALID
+
+
+@pytest.mark.gpu
+def test_a_small_workspace_is_refused_before_anything_is_written(oracle):
+    import ctypes
+
+    from qwen3mk import _cabi
+
+    mk, w, dev = setup(oracle, 35)
+    g = torch.Generator().manual_seed(11)
+    server = Server(2, 16, 20, g)
+    batch = server.batch([3, 5])
+    mk.extend(dev, torch.randint(0, VOCAB, (8,), generator=g).cuda(), batch)
+    k = server.pool.k.clone()
+    ids, nxt = torch.randint(0, VOCAB, (8,), generator=g).cuda(), torch.zeros(2, dtype=torch.int64, device="cuda")
+    need = batch.workspace_bytes(16)
+    space = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for at, size in ((space.data_ptr(), need - 1), (None, need), (space.data_ptr() + 4, need)):
+        a = _cabi.ExtendArgs(ctypes.pointer(batch.view(0)), server.pool.k.stride(0), ids.data_ptr(), None, nxt.data_ptr(), at, size)
+        with pytest.raises(ValueError, match="workspace"):
+            _cabi.check(mk.lib, mk.handle, mk.lib.q3_extend(mk.handle, ctypes.byref(a), None), "q3_extend")
+    torch.cuda.synchronize()
+    assert torch.equal(server.pool.k.view(torch.int16), k.view(torch.int16))
