@@ -261,7 +261,7 @@ typedef struct q3_paged {
  * kv_heads times 1, 2, 4 or 8; q head h reads kv head h / (q_heads / kv_heads).  A token that sees no position, or none with a weight (all
  * scores -inf), gets zeros; a row that it does not see does not touch its result, whatever it holds.  fp32 scores, maxima, sums and
  * accumulators; the probabilities enter the product with V in the pages' type.  q and out: element (token, head, dim) at token * _token + head * _head + dim, 16-byte
- * aligned, strides multiples of 8, at least 128.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
+ * aligned, strides multiples of 8, at least 128; they must not overlap.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
  * `status`: device, 4 words, or NULL: a wait inside the kernel that gives up reports there as in q3_status and leaves NaN in the rows
  * it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
 typedef struct q3_paged_attn_args {
@@ -283,7 +283,7 @@ int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* a, void* stream);
  *     half layout:  y[i] = n[i] c[i] - n[i + r/2] s[i],   y[i + r/2] = n[i + r/2] c[i] + n[i] s[i],      i < r/2 = rotary_dim / 2
  *     interleaved:  y[2i] = n[2i] c[i] - n[2i + 1] s[i],  y[2i + 1] = n[2i + 1] c[i] + n[2i] s[i]
  * in fp32.  q, k and v: element (token, head, dim) at token * _token + head * _head + dim (they may be slices of one row), 16-byte aligned fp32 or 8-byte
- * aligned bf16 / fp16, strides multiples of 4; q_out as q_paged_attn's q.  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
+ * aligned bf16 / fp16, strides multiples of 4; q_out in the pages' type, 8-byte aligned, strides multiples of 4 and at least 128, possibly q itself where the types agree.  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
  * rotary_dim / 2 angles (any scaling of long contexts is in the table).  A token whose position has no row gets NaN (q, k); one without a slot (no page, or
  * kv_len below the number of new tokens) writes no k and v.  `positions`: device [n_tokens] or NULL: rotate by these instead of the tokens' places
  * in their sequences.  q may be NULL (k and v only), and k and v both (q only).  Allocates nothing, no host sync. */

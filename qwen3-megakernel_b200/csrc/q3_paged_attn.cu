@@ -1316,6 +1316,7 @@ extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, voi
     const int group = p->q_heads / c->kv_heads;
     if (p->q_heads < 1 || p->q_heads % c->kv_heads || (group != 1 && group != 2 && group != 4 && group != 8))
         return engine_fail(nullptr, Q3_ERR_INVALID, "%s: %d q heads over %d kv heads: a kv head serves 1, 2, 4 or 8", who, p->q_heads, c->kv_heads);
+    if (p->out == p->q) return bad("out must not be q (rows are read again where a result is not finite)");
     if (!(p->scale > 0.f) || p->scale > 1e30f) return bad("scale must be positive and at most 1e30");
     if ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out) | reinterpret_cast<uintptr_t>(p->workspace)) & 15) return bad("q, out and workspace must be 16-byte aligned");
     const int64_t most = 1ll << 38;

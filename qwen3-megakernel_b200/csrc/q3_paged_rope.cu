@@ -29,8 +29,8 @@ struct PagedRopeArgs {
 };
 
 template <int TYPE> __device__ __forceinline__ float4 rp_load(const unsigned char* p) {       // four elements
-    if constexpr (TYPE == Q3_TYPE_FP32) return __ldg(reinterpret_cast<const float4*>(p));
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+    if constexpr (TYPE == Q3_TYPE_FP32) return *reinterpret_cast<const float4*>(p);       // (not by way of the read-only cache: q_out may be q)
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
     if constexpr (TYPE == Q3_TYPE_BF16) return make_float4(bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y));
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
     return make_float4(a.x, a.y, b.x, b.y);
@@ -173,6 +173,7 @@ extern "C" int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* p, voi
     const int64_t most = 1ll << 38;
     for (int64_t s : {p->q_token, p->q_head, p->k_token, p->k_head, p->v_token, p->v_head, p->out_token, p->out_head})
         if (s < 0 || s > most || s % 4) return bad("strides must be multiples of 4 elements, not negative");
+    if (p->q && ((c->n_tokens > 1 && p->out_token < HEAD_DIM) || (p->q_heads > 1 && p->out_head < HEAD_DIM))) return bad("rows of q_out must not overlap: strides of at least 128");
     PagedRopeArgs a{};
     a.c = paged_view(c);
     a.sh.heads = c->kv_heads; a.sh.batch = c->batch; a.sh.n_tokens = c->n_tokens; a.sh.most_keys = c->table_pages * c->page_size;

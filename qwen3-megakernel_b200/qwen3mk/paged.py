@@ -81,7 +81,7 @@ class PagedBatch:
         self.batch, self.tokens, self.max_new = batch, int(tokens), int(max_new)
         self.lib = _cabi.load()
         self._views: dict = {}
-        self._space = None
+        self._space: dict = {}
 
     def view(self, layer: int) -> _cabi.Paged:
         """The C ABI's descriptor of one layer."""
@@ -98,13 +98,14 @@ class PagedBatch:
         return c
 
     def workspace_bytes(self, q_heads: int) -> int:
-        if self._space is None:
+        n = self._space.get(q_heads)
+        if n is None:
             with _on(self.pool.device):
                 n = self.lib.q3_paged_attn_workspace(self.view(0), q_heads)
             if n < 0:
                 _cabi.check(self.lib, None, int(n), "q3_paged_attn_workspace")
-            self._space = n
-        return self._space
+            self._space[q_heads] = n
+        return n
 
 
 def _strides(what: str, t: torch.Tensor, batch: PagedBatch, dtypes, heads: int | None = None):
@@ -119,7 +120,7 @@ def _strides(what: str, t: torch.Tensor, batch: PagedBatch, dtypes, heads: int |
 def attention(batch: PagedBatch, q: torch.Tensor, layer: int = 0, *, scale: float = HEAD_DIM ** -0.5, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the new tokens over their sequences' pages (whose rows of the new tokens have been written, see rope_append).
 
-    q: [tokens, heads, 128] in the pages' type, heads 1, 2, 4 or 8 times the pool's.  Returns out (q's shape and type).  A token that sees no position gets zeros;
+    q: [tokens, heads, 128] in the pages' type, heads 1, 2, 4 or 8 times the pool's.  Returns out (q's shape and type; not q itself).  A token that sees no position gets zeros;
     rows that a token does not see (later tokens', slots behind the last position) do not touch its result, whatever they hold.  Equal bits on every run."""
     sq = _strides("attention: q", q, batch, batch.dtypes)
     heads = q.shape[1]
@@ -140,7 +141,7 @@ def rope_append(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Te
                 k_gain: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, positions: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """The new tokens' rows: RMS norm of every q and k head (where a gain, bf16 [128], is given), rotary embedding, k and v into the pages.  Returns q's rows in the
-    pages' type (`out` when given), as `attention` reads them.
+    pages' type (`out` when given: q itself where the types agree, say), as `attention` reads them.
 
     q [tokens, heads, 128], k and v [tokens, kv_heads, 128]: fp32, bf16 or fp16, all three alike; slices of one projection's rows serve.  rope: fp32
     [positions, rotary_dim], contiguous, a row the cosines and then the sines (`rope_table`); its width says how many dims of a head are rotated (a multiple of 8

@@ -501,3 +501,33 @@ def test_refusals():
     # no new token at all: nothing to do
     none = describe(pool, table, [0], [20])
     assert paged.attention(none, q[:0]).shape == (0, 16, D)
+
+
+def test_one_batch_serves_q_of_several_head_counts():
+    """The workspace goes by the q heads of the call: 8 new tokens of 16 heads are few rows, of 64 heads many."""
+    from qwen3mk import paged
+
+    g = torch.Generator().manual_seed(24)
+    news, lens = [8, 3], [200, 45]
+    pool, table, rows = make_pool(g, lens, 16, 8, torch.bfloat16)
+    batch = describe(pool, table, news, lens)
+    for heads in (16, 64, 8, 64):
+        q = torch.randn(sum(news), heads, D, generator=g).to(torch.bfloat16).cuda()
+        check(paged.attention(batch, q), q, rows, news, lens)
+
+
+def test_q_in_place_and_outputs_that_overlap():
+    from qwen3mk import paged
+
+    g = torch.Generator().manual_seed(25)
+    pool, table, _ = make_pool(g, [60, 9], 16, 8, torch.bfloat16)
+    batch = describe(pool, table, [33, 9], [60, 9])
+    x = torch.randn(42, 32, D, generator=g).to(torch.bfloat16).cuda()
+    rope, gain = paged.rope_table(64), torch.ones(D, dtype=torch.bfloat16, device="cuda")
+    want = paged.rope_append(batch, x[:, :16], x[:, 16:24], x[:, 24:], rope, q_gain=gain)
+    q = x[:, :16]
+    assert paged.rope_append(batch, q, x[:, 16:24], x[:, 24:], rope, q_gain=gain, out=q) is q and torch.equal(q, want)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.rope_append(batch, q, x[:, 16:24], x[:, 24:], rope, out=want[:1].expand(42, 16, D))
+    with pytest.raises(ValueError, match="out must not be q"):
+        paged.attention(batch, want, out=want)
