@@ -679,7 +679,7 @@ extern "C" int q3_sample_rows(const q3_sample_rows_args* p, void* stream) {
     int cluster = p->batch <= 4 ? 16 : p->batch <= 14 ? 8 : p->batch <= 36 ? 4 : p->batch <= 74 ? 2 : 1;
     while (cluster > 1 && p->vocab < cluster * SR_THREADS) cluster /= 2;
     // N threads of which k hold words beyond a bound hold -N ln(1 - k/N) of them, if words are spread evenly: SR_NUCLEUS leaves the list of SR_LIST room for a bin more
-    // (512 maxima whatever N: 27 mixed rows up to 210 us, where one has a nucleus of 500 words or more; now 43 at most over 200 draws, 25 in the middle)
+    // (512 maxima whatever N: 27 mixed rows up to 210 us, where one has a nucleus of 500 words or more; now 45 at most over 200 draws, 20 in the middle)
     a.nucleus = (int)(cluster * SR_THREADS * (1. - exp(-(double)SR_NUCLEUS / (cluster * SR_THREADS))));
     cudaError_t e = cluster > 8 ? cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : cudaSuccess;
     if (e == cudaSuccess) {
