@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     constexpr int NS = S::NS, GROUPS = PT_GROUPS;
     extern __shared__ __align__(1024) unsigned char pt_raw[];
     __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PT_THREADS / 32];
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[NS], p_full[NS], s_free[NS], o_full[2], o_free, ref_full, l_full[2], drain_bar[2];
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full[2], q_empty[2], s_full[NS], p_full[NS], s_free[NS], o_full[2], o_free, ref_full[2], l_full[2], drain_bar[2];
     __shared__ __align__(8) uint64_t seg_full[PT_RING], seg_empty[PT_RING];
     __shared__ PtSeg s_seg[PT_RING];
     __shared__ uint32_t tmem_base_s;
@@ -547,13 +547,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
             pt_init(&k_full[s], 1); pt_init(&v_full[s], 1); pt_init(&k_empty[s], 1); pt_init(&v_empty[s], 1);
-            pt_init(&q_full[s], 1); pt_init(&q_empty[s], 1); pt_init(&l_full[s], 4);
+            pt_init(&q_full[s], 1); pt_init(&q_empty[s], 1); pt_init(&l_full[s], 4); pt_init(&ref_full[s], 4);
             pt_init(&o_full[s], 1); pt_init(&drain_bar[s], 1);
         }
         for (int s = 0; s < NS; ++s) { pt_init(&s_full[s], 1); pt_init(&p_full[s], 4); pt_init(&s_free[s], 1); }
         for (int s = 0; s < PT_RING; ++s) { pt_init(&seg_full[s], 1); pt_init(&seg_empty[s], 3 + 4 * GROUPS); }
         pt_init(&o_free, 4);
-        pt_init(&ref_full, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
         for (int e = 0; e < 4 * GROUPS; ++e) s_bad[e >> 2][e & 3] = 0;
@@ -808,9 +807,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if constexpr (ONE) {                 // the group of the first tile leaves its m to the others
                     if (t == 0) {
                         __syncwarp();
-                        if (lane == 0) pt_arrive(&ref_full);
+                        if (lane == 0) pt_arrive(&ref_full[n_q & 1]);
                     } else if (t == t0) {
-                        group.wait(&ref_full, (uint32_t)n_q & 1u, 93);
+                        group.wait(&ref_full[n_q & 1], (uint32_t)(n_q >> 1) & 1u, 93);
                         m = s_ref[n_q & 1][row];
                     }
                 }
@@ -857,6 +856,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if (tile0 + PT_KEYS > d.key1) {
                     // rows of V that no row of this tile sees but whose page is there: what they hold is not ours to multiply, even by 0
                     const int rows_log = min(a.c.page_log, 7), z0 = d.key1 - tile0, z1 = min(PT_KEYS, ((z0 + (1 << rows_log) - 1) >> rows_log) << rows_log);
+                    // (with three S a group may be here before V of two tiles ago has landed in this stage, and a barrier that is a phase behind passes for one that is done: first
+                    // that tile's product, which is done once at most before this tile's)
+                    if (ONE && g >= 2) group.wait(&s_free[(g - 2) % NS], (uint32_t)((g - 2) / NS) & 1u, 99);
                     group.wait(&v_full[g & 1], (uint32_t)(g >> 1) & 1u, 90);
                     for (int e = st & 127; e < (z1 - z0) * 16; e += 128)
                         *reinterpret_cast<uint4*>(sKV + (size_t)(g & 1) * 2 * PT_TILE + PT_TILE + (size_t)((e >> 3) & 1) * PT_BOX + (size_t)(z0 + (e >> 4)) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);

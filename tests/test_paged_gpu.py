@@ -531,3 +531,23 @@ def test_q_in_place_and_outputs_that_overlap():
         paged.rope_append(batch, q, x[:, 16:24], x[:, 24:], rope, out=want[:1].expand(42, 16, D))
     with pytest.raises(ValueError, match="out must not be q"):
         paged.attention(batch, want, out=want)
+
+
+@pytest.mark.parametrize("news,lens,page,heads", [([39] * 8, [5527] * 8, 64, 16), ([28] * 15, [3609] * 15, 32, 8), ([43] + [1] * 28, [2032 - 31 * i for i in range(29)], 64, 16),
+                                                   ([130, 131], [700, 2001], 16, 16)])
+def test_pages_that_arrive_late(news, lens, page, heads):
+    """Cold caches: K and V come late and out of step with one another, over and over with the same bits."""
+    from qwen3mk import paged
+
+    g = torch.Generator().manual_seed(26)
+    pool, table, rows = make_pool(g, lens, page, 8, torch.bfloat16)
+    batch = describe(pool, table, news, lens)
+    q = torch.randn(sum(news), heads, D, generator=g).to(torch.bfloat16).cuda()
+    flush = torch.empty(300_000_000, dtype=torch.uint8, device="cuda")
+    first = paged.attention(batch, q)
+    check(first, q, rows, news, lens)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(200):
+        flush.fill_(i & 1)
+        differ += (paged.attention(batch, q).view(torch.int16) != first.view(torch.int16)).any()
+    assert int(differ) == 0
