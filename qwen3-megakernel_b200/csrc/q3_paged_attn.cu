@@ -1136,7 +1136,7 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedAttnA
     }
 }
 
-// The same for results of the tile kernel, whose outputs lie [32 quarters of 16 bytes][128 rows] with the maxima and sums behind them: a lane a row, a warp eight quarters.
+// The same for results of the tile kernel, whose outputs lie [32 quarters of 16 bytes][128 rows] with the maxima and sums behind them: a lane a row, a warp eight quarters (8 answers 39.1 us, 38.2 with two parts at a time).
 template <typename T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_join_tiles_kernel(const PagedAttnArgs a) {
     pdl_launch();
@@ -1162,16 +1162,24 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_tiles_kernel(const Page
     float4 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = stats(i);
-        float4 x[8];
+    for (int i0 = 0; i0 < parts; i0 += 2) {          // two parts' loads under way
+        float4 x[2][8];
+        float2 ml[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = reinterpret_cast<const float4*>(part(i))[(d0 + j) * 128 + row];
-        const float w = ml.x == -INFINITY ? 0.f : ml.x == Ms ? 1.f : pg_ex2(ml.x - Ms);
-        if (w != 0.f) {
-            L = fmaf(ml.y, w, L);
+        for (int i = 0; i < 2; ++i)
+            if (i0 + i < parts) {
+                ml[i] = stats(i0 + i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[j].x = fmaf(x[j].x, w, v[j].x); v[j].y = fmaf(x[j].y, w, v[j].y); v[j].z = fmaf(x[j].z, w, v[j].z); v[j].w = fmaf(x[j].w, w, v[j].w); }
+                for (int j = 0; j < 8; ++j) x[i][j] = reinterpret_cast<const float4*>(part(i0 + i))[(d0 + j) * 128 + row];
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float w = i0 + i >= parts || ml[i].x == -INFINITY ? 0.f : ml[i].x == Ms ? 1.f : pg_ex2(ml[i].x - Ms);
+            if (w != 0.f) {
+                L = fmaf(ml[i].y, w, L);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { v[j].x = fmaf(x[i][j].x, w, v[j].x); v[j].y = fmaf(x[i][j].y, w, v[j].y); v[j].z = fmaf(x[i][j].z, w, v[j].z); v[j].w = fmaf(x[i][j].w, w, v[j].w); }
+            }
         }
     }
     const float r = L > 0.f || L != L ? 1.f / L : 0.f;
