@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
 // behind 8192: 2.3e-3 off, 1.7e-3 of it the output's own rounding (P truncated, as fast: 2.4e-3, and 2.6e-3 with short sequences).
 //
 // Measured: 2048 tokens behind 8192 143 us, 1.08 PFLOP/s of the 1.64 that a large product reaches; 1650 clocks a tile, of which the special-function pipe has 1024 (an exponential a score),
-// the products 1150, the rest are hand-offs.  (Steps: K and V loaded by warps of their own, a thread a row 178; one O, scores two tiles ahead 166; segments worked
-// out ahead 149; masks as bits, O free before its rows are stored 143.  A third group of warps that only writes: 128 registers a thread, 153.)  Few rows: 8 sequences of 13 tokens behind up
+// the products 1150, the rest are hand-offs.  (Steps: K and V loaded by warps of their own, a thread a row 247 -> 211; one O, scores two tiles ahead 208 -> 178;
+// segments worked out ahead, one lane that looks for a group 166 -> 149; masks as bits, O free before its rows are stored 145 -> 143.  A third group of warps that only writes: 128 registers a thread, 153.)  Few rows: 8 sequences of 13 tokens behind up
 // to 5000, fp16, 38 us; the pages at 6.7 TB/s in the steady state (15.9), the rest start, segment ends and join.
 //
 // A wait that gives up lets every later one give up at once (those in which the softmax warps meet are waits like the others); the block then drains what is under way and
