@@ -918,6 +918,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     const int e = min(max((int)(__float_as_uint(sum) >> 23) - 127, -126), 126);
                     r = __uint_as_float((unsigned)(127 - e) << 23);
                     sum *= r; mx += (float)e;
+                } else if (ONE && sum == 0.f) {
+                    mx = -INFINITY;                  // nothing of this part has a weight: what m it would have been taken under is not a maximum that the join may count
                 }
                 // (a partial result's maxima and sums lie behind its outputs, [32 quarters of 16 bytes][128 rows])
                 if (!whole && row < d.rows) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(mx, sum);
