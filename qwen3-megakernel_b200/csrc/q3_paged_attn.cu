@@ -92,56 +92,134 @@ __device__ __forceinline__ unsigned char* pg_o_row(const PagedAttnArgs& a, const
     return a.out + (long long)(s.seq.q0 + (s.r << a.sh.tile_log) + (row >> a.group_log)) * a.o_token + (long long)((s.h << a.group_log) + (row & ((1 << a.group_log) - 1))) * a.o_head;
 }
 
-// A row again, key by key, reading only what it sees: for rows whose result is not finite.  A product adds 0 * v for keys that a row does not see
-// beside those that its tile's later tokens see, and 0 * inf is no number.  Warps of the block take keys in turn (a lane four dims); leaves maximum, sum and
-// output in res[0], res[1], res[4 ..].  `buf` holds 132 floats a warp.  Every thread of WARPS warps
-// calls it, `warp` is its place among them; `sync` is their barrier, and the last thing done.
+__device__ __forceinline__ float pg_max_nan(float a, float b) {      // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// Rows again, key by key, each reading only what it sees: for rows whose result is not finite.  A product adds 0 * v for keys that a row does not see
+// beside those that its tile's later tokens see, and 0 * inf is no number.  PG_REDO rows of a tile at once (row[i] < 0: none), for which a key is fetched once; the
+// warps of the block take keys in turn (a lane four dims).  Leaves a row's maximum, sum and output in res[0], res[1], res[4 ..] of its PG_PART floats.  `buf` holds
+// PG_REDO * PG_PART floats a warp.  Every thread of WARPS warps calls it, `warp` is its place among them; `sync` is their barrier, and the last thing done.
+constexpr int PG_PART = 132;                          // floats of a row of a partial result: maximum, sum, two unused, output
+constexpr int PG_REDO = 4;
 template <typename T, int WARPS, typename Sync>
-__device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment& s, const PgKeys& k, int row, int warp, float* buf, float* res, const Sync& sync) {
+__device__ __noinline__ void pg_redo_rows(const PagedAttnArgs& a, const PgSegment& s, const PgKeys& k, int4 which, int warp, float* buf, float* res, const Sync& sync) {
+    constexpr int R = PG_REDO, AHEAD = 4;            // keys of a warp whose loads are under way
+    static_assert(AHEAD * R == 16 && R == 4, "a pair of lanes a (key, row)");
     const int lane = threadIdx.x & 31, tid = warp * 32 + lane;
-    const uint2 q2 = *reinterpret_cast<const uint2*>(pg_q_row(a, s, row) + lane * 8);
-    const float2 qa = T::unpack(q2.x), qb = T::unpack(q2.y);
-    const int end = min(k.key1, k.qpos0 + (row >> a.group_log) + 1);
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p = k.key0 + warp; p < end; p += WARPS) {
-        const int page = pg_page(a.c, s.b, p);
-        if (page < 0) continue;
-        const long long at = pg_offset(a.c, page, p & ((1 << a.c.page_log) - 1), s.h) + lane * 8;
-        const uint2 kk = *reinterpret_cast<const uint2*>(a.c.k + at), vv = *reinterpret_cast<const uint2*>(a.c.v + at);
-        const float2 ka = T::unpack(kk.x), kb = T::unpack(kk.y), va = T::unpack(vv.x), vb = T::unpack(vv.y);
-        const float x = warp_sum(qa.x * ka.x + qa.y * ka.y + qb.x * kb.x + qb.y * kb.y) * a.scale;
-        if (x == -INFINITY) continue;
-        const float top = x > m || x != x ? x : m, f = m == top ? 1.f : pg_ex2(m - top), e = pg_ex2(x - top);
-        m = top;
-        l = l * f + e;
-        o[0] = o[0] * f + e * va.x; o[1] = o[1] * f + e * va.y; o[2] = o[2] * f + e * vb.x; o[3] = o[3] * f + e * vb.y;
-    }
-    sync();
-    float* mine = buf + warp * 132;
-    if (lane == 0) { mine[0] = m; mine[1] = l; }
+    const int row[R] = {which.x, which.y, which.z, which.w};
+    float2 qa[R], qb[R];
+    float o[R][4];
+    int end[R], stop = k.key0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mine[4 + lane * 4 + i] = o[i];
-    sync();
-    float top = -INFINITY;
-    bool nan = false;
-    for (int w = 0; w < WARPS; ++w) { top = fmaxf(top, buf[w * 132]); nan = nan || buf[w * 132] != buf[w * 132]; }
-    if (nan) top = NAN;
-    float sum = 0.f, v = 0.f;
-    if (warp < 4) {
-        for (int w = 0; w < WARPS; ++w) {
-            const float mw = buf[w * 132];
-            if (mw == -INFINITY) continue;
-            const float f = mw == top ? 1.f : pg_ex2(mw - top);
-            sum += buf[w * 132 + 1] * f;
-            v += buf[w * 132 + 4 + tid] * f;
+    for (int r = 0; r < R; ++r) {
+        const uint2 q2 = *reinterpret_cast<const uint2*>(pg_q_row(a, s, max(row[r], 0)) + lane * 8);
+        qa[r] = T::unpack(q2.x); qb[r] = T::unpack(q2.y);
+        end[r] = row[r] < 0 ? k.key0 : min(k.key1, k.qpos0 + (row[r] >> a.group_log) + 1);
+        stop = max(stop, end[r]);
+        o[r][0] = o[r][1] = o[r][2] = o[r][3] = 0.f;
+    }
+    // lanes 2 j and 2 j + 1 stand for key j / R of the batch and row j % R: they hold that row's maximum and sum
+    const int my_key = lane >> 3, my_row = (lane >> 1) & 3, my_end = my_row == 0 ? end[0] : my_row == 1 ? end[1] : my_row == 2 ? end[2] : end[3];
+    float m = -INFINITY, l = 0.f;
+    for (long long p0 = k.key0 + warp; p0 < stop; p0 += AHEAD * WARPS) {
+        int page[AHEAD];
+        uint2 kk[AHEAD], vv[AHEAD];
+        float x[AHEAD * R];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) page[i] = p0 + i * WARPS < stop ? pg_page(a.c, s.b, (int)p0 + i * WARPS) : -1;
+        if (max(max(page[0], page[1]), max(page[2], page[3])) < 0) continue;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            kk[i] = vv[i] = make_uint2(0u, 0u);
+            if (page[i] < 0) continue;
+            const long long at = pg_offset(a.c, page[i], ((int)p0 + i * WARPS) & ((1 << a.c.page_log) - 1), s.h) + lane * 8;
+            kk[i] = *reinterpret_cast<const uint2*>(a.c.k + at); vv[i] = *reinterpret_cast<const uint2*>(a.c.v + at);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float2 ka = T::unpack(kk[i].x), kb = T::unpack(kk[i].y);
+#pragma unroll
+            for (int r = 0; r < R; ++r) x[i * R + r] = qa[r].x * ka.x + qa[r].y * ka.y + qb[r].x * kb.x + qb[r].y * kb.y;
+        }
+        // sixteen sums over the warp: each step halves what a lane holds
+#pragma unroll
+        for (int half = 8; half > 0; half >>= 1) {
+            const bool upper = lane & (2 * half);
+#pragma unroll
+            for (int j = 0; j < half; ++j) {
+                const float other = __shfl_xor_sync(0xffffffffu, upper ? x[j] : x[j + half], 2 * half);
+                x[j] = (upper ? x[j + half] : x[j]) + other;
+            }
+        }
+        float y = (x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1)) * a.scale;
+        const int my_page = my_key == 0 ? page[0] : my_key == 1 ? page[1] : my_key == 2 ? page[2] : page[3];
+        if (my_page < 0 || p0 + my_key * WARPS >= my_end) y = -INFINITY;
+        const unsigned seen = __ballot_sync(0xffffffffu, y != -INFINITY);
+        float top = pg_max_nan(m, y);
+        top = pg_max_nan(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = pg_max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float ref = top == -INFINITY ? 0.f : top, f = m == top ? 1.f : pg_ex2(m - ref), e = pg_ex2(y - ref);
+        const bool moved = __any_sync(0xffffffffu, m != top);
+        m = top;
+        float sum = e;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        l = l * f + sum;
+        if (moved)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float fr = __shfl_sync(0xffffffffu, f, 2 * r);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[r][d] *= fr;
+            }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float2 va = T::unpack(vv[i].x), vb = T::unpack(vv[i].y);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int from = 2 * (i * R + r);
+                const float w = __shfl_sync(0xffffffffu, e, from);
+                if ((seen >> from) & 1u) { o[r][0] += w * va.x; o[r][1] += w * va.y; o[r][2] += w * vb.x; o[r][3] += w * vb.y; }
+            }
         }
     }
     sync();
-    if (warp < 4) {
-        res[4 + tid] = v;
-        if (tid == 0) { res[0] = top; res[1] = sum; }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float* mine = buf + (warp * R + r) * PG_PART;
+        if (lane == 2 * r) { mine[0] = m; mine[1] = l; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[4 + lane * 4 + i] = o[r][i];
     }
     sync();
+    if (warp < 4)
+        for (int r = 0; r < R; ++r) {
+            const float* const all = buf + r * PG_PART;
+            float top = -INFINITY;
+            bool nan = false;
+            for (int w = 0; w < WARPS; ++w) { const float mw = all[w * R * PG_PART]; top = fmaxf(top, mw); nan = nan || mw != mw; }
+            if (nan) top = NAN;
+            float sum = 0.f, v = 0.f;
+            for (int w = 0; w < WARPS; ++w) {
+                const float mw = all[w * R * PG_PART];
+                if (mw == -INFINITY) continue;
+                const float f = mw == top ? 1.f : pg_ex2(mw - top);
+                sum += all[w * R * PG_PART + 1] * f;
+                v += all[w * R * PG_PART + 4 + tid] * f;
+            }
+            res[r * PG_PART + 4 + tid] = v;
+            if (tid == 0) { res[r * PG_PART] = top; res[r * PG_PART + 1] = sum; }
+        }
+    sync();
+}
+// the next rows of a set that are done again together; they leave it
+__device__ __forceinline__ int4 pg_take_rows(unsigned& set, int first) {
+    int r[PG_REDO];
+#pragma unroll
+    for (int i = 0; i < PG_REDO; ++i) { r[i] = set ? first + __ffs(set) - 1 : -1; set &= set - 1; }
+    return make_int4(r[0], r[1], r[2], r[3]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
@@ -156,7 +234,6 @@ __device__ __noinline__ void pg_redo_row(const PagedAttnArgs& a, const PgSegment
 constexpr int PR_WARPS = 4, PR_THREADS = PR_WARPS * 32, PR_TILE = 16, PR_STAGES = 3, PR_HALF = PR_TILE * 256, PR_STAGE = 2 * PR_HALF;
 constexpr int PR_UNIT_LOG = 6;                        // 64 keys a unit: a tile of 16 for every warp
 constexpr size_t PR_SMEM = (size_t)PR_WARPS * PR_STAGES * PR_STAGE;
-constexpr int PG_PART = 132;                          // floats of a row of a partial result: maximum, sum, two unused, output
 
 __device__ __forceinline__ uint32_t pg_transpose(uint32_t w) {
     uint32_t d;
@@ -173,7 +250,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
     __shared__ long long s_prefix[PG_MAX_BATCH + 1], s_sum[PR_WARPS];
     __shared__ float s_m[PR_WARPS][COLS], s_l[PR_WARPS][COLS];
     __shared__ unsigned s_bad;
-    __shared__ float s_res[132];
+    __shared__ float s_res[PG_REDO * PG_PART];
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp();
     const int fg = lane >> 2, ft = lane & 3, lrow = lane & 7, lmat = lane >> 3;
     pdl_launch();
@@ -370,12 +447,15 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
         }
         __syncthreads();
         auto sync = [] { __syncthreads(); };
-        for (unsigned bad = s_bad; bad; bad &= bad - 1) {
-            const int row = __ffs(bad) - 1;
+        for (unsigned bad = s_bad; bad;) {
+            const int4 which = pg_take_rows(bad, 0);
             const PgSegment seg = s;                 // (copies: what a call is handed by address would live in memory all along)
             const PgKeys keys = k;
-            pg_redo_row<T, PR_WARPS>(a, seg, keys, row, warp, reinterpret_cast<float*>(pr_raw), s_res, sync);
-            store(row, s_res[0], s_res[1], s_res[4 + tid]);
+            pg_redo_rows<T, PR_WARPS>(a, seg, keys, which, warp, reinterpret_cast<float*>(pr_raw), s_res, sync);
+            const int row[PG_REDO] = {which.x, which.y, which.z, which.w};
+#pragma unroll
+            for (int i = 0; i < PG_REDO; ++i)
+                if (row[i] >= 0) store(row[i], s_res[i * PG_PART], s_res[i * PG_PART + 1], s_res[i * PG_PART + 4 + tid]);
         }
         __syncthreads();
         if (tid == 0) {
@@ -398,7 +478,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
 //
 // bf16: P has fp32's exponents, so that m need not be the maximum: the largest score of the segment's first tile (0 where a row sees none of it) serves all its
 // tiles.  Nothing is rescaled, no other tile is searched for its maximum, one O serves all groups, and there is room for three S.  A row that leaves fp32's range (scores 88 above the first tile's) is not finite at the end, one that has vanished (no weight
-// above 2^-100 though it sees keys) is seen by its sum: both are done again row by row.
+// above 2^-100 though it sees keys) is seen by its sum: both are marked, and done again row by row once the block's run is over and nobody waits any more.
 // fp16: P must not leave [2^-24, 2^16), so m follows a group's maximum, and its O is rescaled when a score exceeds m by 2^8; two S and two O.
 // P is rounded to the pages' type and its sum is that of the rounded values: where few keys hold a row's weight their roundings leave the quotient.  2048 tokens
 // behind 8192: 2.3e-3 off, 1.7e-3 of it the output's own rounding (P truncated, as fast: 2.4e-3, and 2.6e-3 with short sequences).
@@ -512,11 +592,7 @@ struct PtGroup {
         sync();
     }
 };
-// the group's own, for pg_redo_row
-struct PtSync {
-    const PtGroup& group;
-    __device__ __forceinline__ void operator()() const { group.sync(); }
-};
+constexpr uint32_t PT_AGAIN = 0x7fff7fffu;                    // what a finished row begins with that is to be done again (finished rows hold no NaN)
 
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -533,10 +609,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     __shared__ volatile int abort_flag;
     __shared__ float s_ref[2][128];                 // ONE: what a row's P is taken under, by the segment's parity
     __shared__ float s_m[2][128], s_l[2][128];      // what the group that does not write a segment's rows leaves to the other: maximum (fp16) and sum, by the segment's parity
-    __shared__ float s_room[4 * 132];               // of pg_redo_row
-    __shared__ unsigned s_bad[GROUPS][4];           // per group: rows that are done again
+    __shared__ unsigned s_again[4];                 // rows of a segment that are done again, once the run is over
+    __shared__ int s_any;                           // whether there are any
     __shared__ int s_ok[GROUPS];                      // per group: what its first warp has decided for all four
-    __shared__ float s_res[132];
+    __shared__ float s_res[PG_REDO * PG_PART];
 
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     if (tid < 96 && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(warp == 0 ? &tm_q : warp == 1 ? &tm_k : &tm_v) : "memory");
@@ -561,7 +637,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         pt_init(&o_free, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
-        for (int e = 0; e < 4 * GROUPS; ++e) s_bad[e >> 2][e & 3] = 0;
+        s_any = 0;
     }
     if (warp == PT_MMA_O) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&tmem_base_s)), "r"(512u) : "memory");
@@ -1006,30 +1082,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 }
                 const float2 odd2 = pt_unpair(odd);
                 bad = (bad || odd2.x != 0.f || odd2.y != 0.f) && row < d.rows;
-                const unsigned again = __ballot_sync(0xffffffffu, bad);
-                if (lane == 0) s_bad[grp][quad] = again;
-                __syncwarp();
-                group.sync();
-                if (s_bad[grp][0] | s_bad[grp][1] | s_bad[grp][2] | s_bad[grp][3]) {
-                    PgSegment seg{};                 // (what pg_redo_row asks of it)
-                    seg.b = d.b; seg.h = d.h; seg.seq.q0 = d.q_row;
-                    const PgKeys keys{d.key0, d.key1, d.qpos0, d.rows};
-                    PtSync sync{group};
-                    for (int q = 0; q < 4; ++q)
-                        for (unsigned b = s_bad[grp][q]; b; b &= b - 1) {
-                            const int rr = q * 32 + __ffs(b) - 1;
-                            // (the groups write in turn: a segment's rows are finished before the next one's are looked at, so one room serves both)
-                            pg_redo_row<T, 4>(a, seg, keys, rr, quad, s_room, s_res, sync);
-                            const int dim = quad * 32 + lane;
-                            const float L = s_res[1], inv = L > 0.f || L != L ? 1.f / L : 0.f, x = s_res[4 + dim], up = __shfl_down_sync(0xffffffffu, x, 1);
-                            if (whole) {
-                                if (!(dim & 1)) *reinterpret_cast<uint32_t*>(pg_o_row(a, seg, rr) + dim * 2) = T::pack(x * inv, up * inv);
-                            } else {
-                                parts[((dim >> 2) * 128 + rr) * 4 + (dim & 3)] = x;
-                                if (dim == 0) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[rr] = make_float2(s_res[0], L);
-                            }
-                            group.sync();
-                        }
+                if (bad) {                           // marked, and done again when nobody waits any more
+                    if (whole) *reinterpret_cast<uint32_t*>(o_row) = PT_AGAIN;
+                    else reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(NAN, NAN);
+                    s_any = 1;
                 }
             }
             if (n > 0) {
@@ -1053,6 +1109,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             tc_drain(&drain_bar[warp == PT_MMA_S], 0);
         }
         __syncthreads();
+    }
+    if (warp == PT_MMA_O) {                          // (before the rows that are done again: another kernel's block may be waiting for columns)
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+    if (abort_flag) {
         PgWalk w;
         bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
         while (left) {
@@ -1066,11 +1129,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             first = false;
             left = w.next(a.sh, qs, kl);
         }
-    }
-    if (warp == PT_MMA_O) {
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    } else if (s_any) {
+        // The run is over, its memory is free and no wait depends on how long this takes: the marked rows, all warps at their keys.  (64 tokens of 16 heads behind
+        // 33000 positions, whose last V row holds an infinity: 2.2 ms instead of 70 us; 2048 behind 8192 with scores that rise by 120: 19 ms instead of 170 us.)
+        float* const room = reinterpret_cast<float*>(pt_raw);
+        auto sync = [] { __syncthreads(); };
+        PgWalk w;
+        bool left = w.begin(a.sh, s_prefix, qs, kl, from, to), first = true;
+        while (left) {
+            const PgSegment seg = w.s;
+            const PgKeys keys = pg_keys(a, seg);
+            const bool whole = w.whole();
+            float* const parts = a.part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * 128 * PG_PART;
+            float2* const stats = reinterpret_cast<float2*>(parts + 128 * HEAD_DIM);
+            if (warp < 4) {
+                bool bad = tid < keys.rows;
+                if (bad) bad = whole ? *reinterpret_cast<const uint32_t*>(pg_o_row(a, seg, tid)) == PT_AGAIN : stats[tid].x != stats[tid].x;
+                const unsigned again = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0) s_again[warp] = again;
+            }
+            __syncthreads();
+            for (int q = 0; q < 4; ++q)
+                for (unsigned set = s_again[q]; set;) {
+                    const int4 which = pg_take_rows(set, q * 32);
+                    pg_redo_rows<T, PT_THREADS / 32>(a, seg, keys, which, warp, room, s_res, sync);
+                    const int row[PG_REDO] = {which.x, which.y, which.z, which.w};
+                    if (warp < 4)
+#pragma unroll
+                        for (int i = 0; i < PG_REDO; ++i) {
+                            const int rr = row[i];
+                            const float* const done = s_res + i * PG_PART;
+                            const float L = done[1], inv = L > 0.f || L != L ? 1.f / L : 0.f, x = done[4 + tid], up = __shfl_down_sync(0xffffffffu, x, 1);
+                            if (rr < 0) continue;
+                            if (whole) {
+                                if (!(tid & 1)) *reinterpret_cast<uint32_t*>(pg_o_row(a, seg, rr) + tid * 2) = T::pack(x * inv, up * inv);
+                            } else {
+                                parts[((tid >> 2) * 128 + rr) * 4 + (tid & 3)] = x;
+                                if (tid == 0) stats[rr] = make_float2(done[0], L);
+                            }
+                        }
+                }
+            __syncthreads();                         // (the marks have been read)
+            first = false;
+            left = w.next(a.sh, qs, kl);
+        }
     }
 }
 
