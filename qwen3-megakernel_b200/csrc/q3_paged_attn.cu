@@ -728,10 +728,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if (left) {
                     const PgKeys k = pg_keys(a, w.s);
                     d = PtSeg{(k.key1 - k.key0 + PT_KEYS - 1) / PT_KEYS, w.s.b, w.s.h, w.s.seq.q0 + (w.s.r << a.sh.tile_log), k.key0, k.key1, k.qpos0, k.rows, w.whole(), 1};
-                    bool every = true;               // all pages of the segment are there
-                    for (int e = (k.key0 >> a.c.page_log) + lane; d.n > 0 && e <= (k.key1 - 1) >> a.c.page_log; e += 32)
-                        every = every && (unsigned)a.c.table[(long long)d.b * a.c.table_stride + e] < (unsigned)a.c.n_pages;
+                    bool every = true, some = false;         // all pages of the segment are there; at least one is
+                    for (int e = (k.key0 >> a.c.page_log) + lane; d.n > 0 && e <= (k.key1 - 1) >> a.c.page_log; e += 32) {
+                        const bool there = (unsigned)a.c.table[(long long)d.b * a.c.table_stride + e] < (unsigned)a.c.n_pages;
+                        every = every && there; some = some || there;
+                    }
                     d.every = __all_sync(0xffffffffu, every);
+                    if (!__any_sync(0xffffffffu, some)) d.n = 0;             // (a segment without a page, of a caller who drops old ones: as if it had no keys)
                 }
                 if (i >= PT_RING && !pt_wait_warp<true>(&seg_empty[i % PT_RING], (uint32_t)(i / PT_RING - 1) & 1u, &abort_flag, a.status, 96)) break;
                 if (lane == 0) {

@@ -85,3 +85,38 @@ def test_few_rows_behind_a_long_cache(new):
     pool.v[0, at, s, :, 3] = float("inf")
     rows[0][1][n - 1, :, 3] = float("inf")
     check(paged.attention(describe(pool, table, [new, new], [n, n]), q), q, rows, [new, new], [n, n])
+
+
+def median_us(f, runs=9):
+    f()
+    times = []
+    for _ in range(runs):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return sorted(times)[runs // 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kept", [0, 1000])
+def test_pages_that_are_gone_cost_nothing(dtype, kept):
+    """A caller who drops old pages: what is left is attended, and the call takes no longer than with all of them (before, a row that found nothing in a part looked
+    for its keys one by one: fifty times as long)."""
+    from qwen3mk import paged
+
+    g = torch.Generator().manual_seed(204)
+    new, n, page = 64, 33064, 64
+    pool, table, rows = make_pool(g, [n], page, 8, dtype)
+    q = torch.randn(new, 16, D, generator=g).to(dtype).cuda()
+    batch = describe(pool, table, [new], [n])
+    whole = median_us(lambda: paged.attention(batch, q))
+    gone = (n - kept) // page if kept else table.shape[1]
+    table[0, :gone] = -1
+    out = paged.attention(batch, q)
+    there = [torch.arange(n, device="cuda") >= gone * page]
+    check(out, q, rows, [new], [n], there=there)
+    less = median_us(lambda: paged.attention(batch, q))
+    assert less < 2 * whole, f"{less:.0f} us without {gone} pages, {whole:.0f} us with them"
