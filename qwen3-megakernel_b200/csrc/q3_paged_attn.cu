@@ -498,6 +498,7 @@ template <typename T> struct PtShape {
     static constexpr int NS = ONE ? 3 : 2;                    // buffers of S and P
 };
 constexpr int PT_RING = 4;                                    // segments that have been worked out ahead
+constexpr int PT_SCAN = 1 << 15;                              // entries of the page table that are looked at for that: 1024 loads a lane, a millisecond at most of the 200 that a wait has
 constexpr int PT_GROUPS = 2, PT_THREADS = 32 * PT_FIRST + PT_GROUPS * 128;
 struct PtSeg { int n, b, h, q_row, key0, key1, qpos0, rows, whole, every; };      // n tiles of one item's keys; n < 0: the run is over
 constexpr int PT_KEYS = 128;                                  // keys of a tile, the unit of work
@@ -729,7 +730,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     const PgKeys k = pg_keys(a, w.s);
                     d = PtSeg{(k.key1 - k.key0 + PT_KEYS - 1) / PT_KEYS, w.s.b, w.s.h, w.s.seq.q0 + (w.s.r << a.sh.tile_log), k.key0, k.key1, k.qpos0, k.rows, w.whole(), 1};
                     bool every = true, some = false;         // all pages of the segment are there; at least one is
-                    for (int e = (k.key0 >> a.c.page_log) + lane; d.n > 0 && e <= (k.key1 - 1) >> a.c.page_log; e += 32) {
+                    const int e0 = k.key0 >> a.c.page_log, e1 = d.n > 0 ? ((k.key1 - 1) >> a.c.page_log) + 1 : e0;
+                    const bool known = e1 - e0 <= PT_SCAN;                   // (of more pages every tile looks for its own: the others wait for this)
+                    if (!known) { every = false; some = true; }
+                    for (int e = e0 + lane; known && e < e1; e += 32) {
                         const bool there = (unsigned)a.c.table[(long long)d.b * a.c.table_stride + e] < (unsigned)a.c.n_pages;
                         every = every && there; some = some || there;
                     }
