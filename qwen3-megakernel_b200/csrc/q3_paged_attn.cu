@@ -612,7 +612,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     __shared__ float s_m[2][128], s_l[2][128];      // what the group that does not write a segment's rows leaves to the other: maximum (fp16) and sum, by the segment's parity
     __shared__ unsigned s_again[4];                 // rows of a segment that are done again, once the run is over
     __shared__ int s_any;                           // whether there are any
-    __shared__ int s_ok[GROUPS];                      // per group: what its first warp has decided for all four
+    __shared__ int s_ok[GROUPS][2];                   // per group: what its first warp has decided for all four, by the segment's parity (a group without a tile of a segment meets once in it:
+                                                      // its first warp may be at the next decision before the others have read this one)
     __shared__ float s_res[PG_REDO * PG_PART];
 
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
@@ -824,10 +825,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         bool first = true;
         int g0 = 0, n_q = 0;                         // number of the segment's first tile; segments with tiles
         for (int i = 0;; ++i) {
-            if (quad == 0 && lane == 0) s_ok[grp] = pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 97);
+            if (quad == 0 && lane == 0) s_ok[grp][i & 1] = pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 97);
             __syncwarp();
             group.sync();
-            if (!s_ok[grp]) break;
+            if (!s_ok[grp][i & 1]) break;
             const PtSeg d = s_seg[i % PT_RING];
             __syncwarp();
             if (lane == 0) pt_arrive(&seg_empty[i % PT_RING]);
