@@ -53,7 +53,7 @@ typedef struct q3_config {
     int32_t max_batch;      /* largest q3_decode_args.batch the scratch is sized for (>= 1)      */
     int32_t max_tokens;     /* largest q3_prefill_args.n_tokens the scratch is sized for (0: no prefill) */
     int32_t grid_limit;     /* 0 = one CTA per SM; otherwise cap the persistent grid (tests)     */
-    int32_t wait_limit_us;  /* patience of the persistent and the layer kernel's waits in microseconds; 0 = the default (200 ms).  Tests set it low
+    int32_t wait_limit_us;  /* patience of the persistent and the layer kernel's waits, and of q3_extend's attention, in microseconds; 0 = the default (200 ms).  Tests set it low
                                to see a wait give up.  Waits inside the tensor-core products are fixed at 200 ms, at 400 for a cluster's partial tiles */
 } q3_config;
 
@@ -262,8 +262,8 @@ typedef struct q3_paged {
  * scores -inf), gets zeros; a row that it does not see does not touch its result, whatever it holds.  fp32 scores, maxima, sums and
  * accumulators; the probabilities enter the product with V in the pages' type.  q and out: element (token, head, dim) at token * _token + head * _head + dim, 16-byte
  * aligned, strides multiples of 8, at least 128; they must not overlap.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
- * `status`: device, 4 words, or NULL: a wait inside the kernel that gives up reports there as in q3_status and leaves NaN in the rows
- * it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
+ * `status`: device, 4 words that are 0, or NULL: a wait inside the kernel that gives up reports there as in q3_status (the first one since they were 0) and leaves NaN
+ * in the rows it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
 typedef struct q3_paged_attn_args {
     const void* q;
     void* out;
@@ -276,6 +276,8 @@ typedef struct q3_paged_attn_args {
 } q3_paged_attn_args;
 int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads);   /* bytes; depends on the device, the head counts and max_new alone, negative: an error code */
 int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* a, void* stream);
+/* The same with the patience of the kernel's waits in microseconds (0: the default, 200 ms), as q3_config has it for an engine.  Tests set it low to see a wait give up. */
+int q3_paged_attn_limited(const q3_paged* c, const q3_paged_attn_args* a, int32_t wait_limit_us, void* stream);
 
 /* The new tokens' q, k and v rows on their way to that attention: RMS norm of every q and k head (where a gain is given), rotary embedding of its
  * first rotary_dim dims by the table row of the token's position, and the k and v rows rounded once into the slots of their pages:

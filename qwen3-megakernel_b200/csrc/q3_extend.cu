@@ -124,7 +124,7 @@ extern "C" int q3_extend(q3_engine* e, const q3_extend_args* a, void* stream) {
         q3_paged_attn_args t{};
         t.q = q; t.out = attn; t.q_token = t.out_token = Q_DIM; t.q_head = t.out_head = HEAD_DIM; t.q_heads = Q_HEADS; t.scale = ATTN_SCALE;
         t.workspace = a->workspace; t.workspace_bytes = a->workspace_bytes; t.status = e->status;
-        if (rc == Q3_OK) rc = q3_paged_attn(&pl, &t, stream);
+        if (rc == Q3_OK) rc = q3_paged_attn_limited(&pl, &t, e->cfg.wait_limit_us, stream);
         if (rc != Q3_OK) return fail(e, rc, "q3_extend: %s", q3_last_error(nullptr));
         e->launches += 3;
 

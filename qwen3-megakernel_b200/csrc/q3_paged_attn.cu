@@ -30,6 +30,8 @@ struct PagedAttnArgs {
     float* part;                     // two partial results a block
     int least;                       // units a block takes at least
     uint32_t* status;
+    unsigned long long wait_ns;      // how long a wait of the tile kernel lasts at most,
+    unsigned wait_looks;             // and at which looks at the barrier it asks for the time (a mask of their number)
 };
 
 // What a block leaves behind: the item that is cut at its end and began in its run, to be put together of the results of `parts` blocks (0: none)
@@ -509,7 +511,7 @@ constexpr float PT_LAG = 8.f;
 // The thread looks at the barrier without being parked: a tile has eight hand-offs.
 // PARK: it may sleep up to 20 us between two looks (it wakes when the phase completes).
 template <bool PARK = false>
-__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const PagedAttnArgs& a, uint32_t site) {
     unsigned it = 0;
     unsigned long long t0 = 0;
     for (;;) {
@@ -522,11 +524,11 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
                          : "=r"(ok) : "r"(tc_smem(bar)), "r"(parity) : "memory");
         if (ok) return true;
         if (*abort_flag) return false;
-        if ((++it & 63u) == 0) {
+        if ((++it & a.wait_looks) == 0) {
             const unsigned long long t = tc_ns();
             if (t0 == 0) t0 = t;
-            else if (t - t0 > TC_WAIT_NS) {
-                if (status) report(status, ST_MBAR_TIMEOUT, site, parity);
+            else if (t - t0 > a.wait_ns) {
+                if (a.status) report(a.status, ST_MBAR_TIMEOUT, site, parity);
                 *abort_flag = 1;
                 return false;
             }
@@ -534,8 +536,8 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
     }
 }
 template <bool PARK = false>
-__device__ __forceinline__ bool pt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status, uint32_t site) {
-    return one_lane_waits([&] { return pt_wait<PARK>(bar, parity, abort_flag, status, site); });
+__device__ __forceinline__ bool pt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const PagedAttnArgs& a, uint32_t site) {
+    return one_lane_waits([&] { return pt_wait<PARK>(bar, parity, abort_flag, a, site); });
 }
 // MN-major operand: rows are keys (the K index), 64 dims a row; the next 64 dims a box further, the next 8 keys 1024 bytes
 __device__ __forceinline__ uint64_t pt_desc_mn(uint32_t smem_addr) {
@@ -585,10 +587,10 @@ __device__ __forceinline__ void pt_commit(uint64_t* bar) {
 struct PtGroup {
     int grp, quad, lane;
     volatile int* abort_flag;
-    uint32_t* status;
+    const PagedAttnArgs& a;
     __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, 128;" ::"r"(2 + grp) : "memory"); }
     __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, uint32_t site) const {
-        if (quad == 0 && lane == 0) pt_wait(bar, parity, abort_flag, status, site);
+        if (quad == 0 && lane == 0) pt_wait(bar, parity, abort_flag, a, site);
         __syncwarp();
         sync();
     }
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     auto segment = [&](int i) {
         PtSeg d;
         d.n = -1;
-        if (pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 95)) {
+        if (pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a, 95)) {
             d = s_seg[i % PT_RING];
             pt_arrive(&seg_empty[i % PT_RING]);
         }
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
     auto segment_warp = [&](int i) {
         PtSeg d;
         d.n = -1;
-        if (pt_wait_warp<true>(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 95)) {
+        if (pt_wait_warp<true>(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a, 95)) {
             d = s_seg[i % PT_RING];
             __syncwarp();
             if (lane == 0) pt_arrive(&seg_empty[i % PT_RING]);
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             int next = d.n > 0 ? entry(0) : -1;
             if (d.n > 0 && !is_v) {
                 const int buf = n_q & 1;
-                if (n_q >= 2 && !pt_wait_warp<true>(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a.status, 80)) return false;
+                if (n_q >= 2 && !pt_wait_warp<true>(&q_empty[buf], ((n_q >> 1) - 1) & 1, &abort_flag, a, 80)) return false;
                 if (lane == 0) {
                     pt_expect(&q_full[buf], PT_TILE);
 #pragma unroll
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 const int s = g & 1, slot = (key0 + t * PT_KEYS) & ((1 << a.c.page_log) - 1);
                 const int page = (unsigned)next < (unsigned)a.c.n_pages ? next : a.c.n_pages;      // no such page: outside the tensor
                 if (t + 1 < d.n) next = entry(t + 1);  // (on its way while this tile is waited for)
-                if (g >= 2 && !pt_wait_warp<true>(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a.status, 81)) return false;
+                if (g >= 2 && !pt_wait_warp<true>(&empty[s], ((g >> 1) - 1) & 1, &abort_flag, a, 81)) return false;
                 if (lane == 0) pt_expect(&full[s], PT_TILE);
                 __syncwarp();
                 if (mine)
@@ -741,7 +743,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                     d.every = __all_sync(0xffffffffu, every);
                     if (!__any_sync(0xffffffffu, some)) d.n = 0;             // (a segment without a page, of a caller who drops old ones: as if it had no keys)
                 }
-                if (i >= PT_RING && !pt_wait_warp<true>(&seg_empty[i % PT_RING], (uint32_t)(i / PT_RING - 1) & 1u, &abort_flag, a.status, 96)) break;
+                if (i >= PT_RING && !pt_wait_warp<true>(&seg_empty[i % PT_RING], (uint32_t)(i / PT_RING - 1) & 1u, &abort_flag, a, 96)) break;
                 if (lane == 0) {
                     s_seg[i % PT_RING] = d;
                     pt_arrive(&seg_full[i % PT_RING]);
@@ -765,9 +767,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if (n < 0) break;
                 for (int t = 0; t < n; ++t, ++g) {
                     const int s = g & 1, buf = n_q & 1;
-                    if (t == 0) ok = pt_wait(&q_full[buf], (n_q >> 1) & 1, &abort_flag, a.status, 83);
-                    ok = ok && pt_wait(&k_full[s], (g >> 1) & 1, &abort_flag, a.status, 84);
-                    if (use > 0) ok = ok && pt_wait(&s_free[b], (use - 1) & 1, &abort_flag, a.status, 92);      // P of the tile before in this buffer has been multiplied
+                    if (t == 0) ok = pt_wait(&q_full[buf], (n_q >> 1) & 1, &abort_flag, a, 83);
+                    ok = ok && pt_wait(&k_full[s], (g >> 1) & 1, &abort_flag, a, 84);
+                    if (use > 0) ok = ok && pt_wait(&s_free[b], (use - 1) & 1, &abort_flag, a, 92);      // P of the tile before in this buffer has been multiplied
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t dqs = dq + (uint64_t)buf * TILE, dks = dk + (uint64_t)s * 2 * TILE;
@@ -797,8 +799,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 if (n < 0) break;
                 for (int t = 0; t < n; ++t, ++g) {
                     const int s = g & 1;
-                    if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a.status, 85);      // the rows of the segment before have been read
-                    ok = ok && pt_wait(&v_full[s], (g >> 1) & 1, &abort_flag, a.status, 87) && pt_wait(&p_full[b], use & 1, &abort_flag, a.status, 86);
+                    if (t == 0 && seg > 0) ok = pt_wait(&o_free, (seg - 1) & 1, &abort_flag, a, 85);      // the rows of the segment before have been read
+                    ok = ok && pt_wait(&v_full[s], (g >> 1) & 1, &abort_flag, a, 87) && pt_wait(&p_full[b], use & 1, &abort_flag, a, 86);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t dvs = dv + (uint64_t)s * 2 * TILE;
@@ -821,11 +823,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         // ---------------------------------------------------------------------- softmax and output: row = TMEM lane
         const int quad = warp & 3, row = quad * 32 + lane, grp = (warp >> 2) - 1, st = tid - 32 * PT_FIRST;
         const uint32_t trow = tmem_base + ((uint32_t)(quad * 32) << 16);
-        const PtGroup group{grp, quad, lane, &abort_flag, a.status};
+        const PtGroup group{grp, quad, lane, &abort_flag, a};
         bool first = true;
         int g0 = 0, n_q = 0;                         // number of the segment's first tile; segments with tiles
         for (int i = 0;; ++i) {
-            if (quad == 0 && lane == 0) s_ok[grp][i & 1] = pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a.status, 97);
+            if (quad == 0 && lane == 0) s_ok[grp][i & 1] = pt_wait(&seg_full[i % PT_RING], (uint32_t)(i / PT_RING) & 1u, &abort_flag, a, 97);
             __syncwarp();
             group.sync();
             if (!s_ok[grp][i & 1]) break;
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                             if (raise) m = top;
                             lsum *= c;
                             if (t >= GROUPS) {       // O of the group's tiles so far, once the last of them has been added
-                                pt_wait_warp(&o_full[grp], (uint32_t)((g >> 1) - 1) & 1u, &abort_flag, a.status, 89);      // (not every warp of the group comes here)
+                                pt_wait_warp(&o_full[grp], (uint32_t)((g >> 1) - 1) & 1u, &abort_flag, a, 89);      // (not every warp of the group comes here)
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                                 for (int h = 0; h < 128; h += 16) {
@@ -1434,13 +1436,16 @@ extern "C" int64_t q3_paged_attn_workspace(const q3_paged* c, int32_t q_heads) {
     return pg_cut_bytes() + (int64_t)2 * sms * (pg_few(c->max_new, group) ? 2 * 16 : 128) * PG_PART * 4;
 }
 
-extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, void* stream) {
+extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, void* stream) { return q3_paged_attn_limited(c, p, 0, stream); }
+extern "C" int q3_paged_attn_limited(const q3_paged* c, const q3_paged_attn_args* p, int32_t wait_limit_us, void* stream) {
     const char* who = "q3_paged_attn";
     if (const int rc = paged_check(who, c)) return rc;
     auto bad = [&](const char* what) { return engine_fail(nullptr, Q3_ERR_INVALID, "%s: %s", who, what); };
     if (!p) return bad("null argument");
+    if (wait_limit_us < 0) return bad("wait_limit_us must not be negative");
     if (c->n_tokens == 0) return Q3_OK;
     if (!p->q || !p->out || !p->workspace) return bad("q, out and workspace are required");
+    if (reinterpret_cast<uintptr_t>(p->status) & 3) return bad("status must be 4-byte aligned");
     const int group = p->q_heads / c->kv_heads;
     if (p->q_heads < 1 || p->q_heads % c->kv_heads || (group != 1 && group != 2 && group != 4 && group != 8))
         return engine_fail(nullptr, Q3_ERR_INVALID, "%s: %d q heads over %d kv heads: a kv head serves 1, 2, 4 or 8", who, p->q_heads, c->kv_heads);
@@ -1465,6 +1470,8 @@ extern "C" int q3_paged_attn(const q3_paged* c, const q3_paged_attn_args* p, voi
     a.cuts = static_cast<PgCut*>(p->workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + pg_cut_bytes());
     a.status = p->status;
+    a.wait_ns = wait_limit_us > 0 ? (unsigned long long)wait_limit_us * 1000ull : TC_WAIT_NS;
+    a.wait_looks = wait_limit_us > 0 && wait_limit_us < 100 ? 0u : 63u;      // (64 looks take 3 us)
     cudaStream_t st = (cudaStream_t)stream;
     const int max_new = c->max_new < 1 ? 1 : c->max_new;
     const cudaError_t err = c->type == Q3_TYPE_BF16 ? launch_attn<PgBf16>(a, max_new, p->q_heads, st) : launch_attn<PgFp16>(a, max_new, p->q_heads, st);

@@ -50,6 +50,17 @@ class PagePool:
         self.k, self.v = k, v
         self.layers, self.pages, self.page_size, self.kv_heads = (int(x) for x in k.shape[:4])
         self.device, self.dtype = k.device, k.dtype
+        self._status = torch.zeros(4, dtype=torch.int32, device=k.device)      # what `attention` reports of a wait that gave up
+
+    def status(self, stream: torch.cuda.Stream | None = None) -> list[int]:
+        """Synchronise the (current) stream and read the status words of `attention` over this pool; raises RuntimeError, and clears them, if a wait inside a kernel gave
+        up: rows of that call are NaN.  (`Megakernel.extend` reports to `Megakernel.status`.)"""
+        (torch.cuda.current_stream(self.device) if stream is None else stream).synchronize()
+        words = self._status.tolist()
+        if words[0]:
+            self._status.zero_()
+            raise RuntimeError(f"paged attention: device status: code {words[0]} at site {words[1]}, CTA {words[2]}, value {words[3]}")
+        return words
 
     @classmethod
     def empty(cls, *, layers: int = 28, pages: int, page_size: int = 64, kv_heads: int = 8, dtype=torch.bfloat16, device="cuda") -> "PagePool":
@@ -62,9 +73,10 @@ class PagedBatch:
 
     tokens: rows of q (default: q_start[-1]); rows behind the last sequence's are left as they were.  max_new: most new tokens of a sequence, which
     chooses the kernels and bounds nothing (default: read from q_start).  Both defaults read q_start on the host, once, here.  The tensors are kept
-    and may be changed in place between calls."""
+    and may be changed in place between calls.  wait_limit_us: patience of the waits inside `attention`'s kernel (0: 200 ms), as an engine has it; tests set it low."""
 
-    def __init__(self, pool: PagePool, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *, tokens: int | None = None, max_new: int | None = None):
+    def __init__(self, pool: PagePool, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *, tokens: int | None = None, max_new: int | None = None,
+                 wait_limit_us: int = 0):
         batch = kv_len.numel()
         for name, t, ok in (("page_table", page_table, page_table.dim() == 2 and page_table.shape[0] == batch and (page_table.shape[1] == 1 or page_table.stride(1) == 1)),
                             ("q_start", q_start, q_start.shape == (batch + 1,) and q_start.is_contiguous()),
@@ -79,6 +91,7 @@ class PagedBatch:
         self.pool, self.page_table, self.q_start, self.kv_len = pool, page_table, q_start, kv_len
         self.device, self.dtypes = pool.device, (pool.dtype,)
         self.batch, self.tokens, self.max_new = batch, int(tokens), int(max_new)
+        self.wait_limit_us, self._status = int(wait_limit_us), pool._status.data_ptr()
         self.lib = _cabi.load()
         self._views: dict = {}
         self._space: dict = {}
@@ -121,7 +134,8 @@ def attention(batch: PagedBatch, q: torch.Tensor, layer: int = 0, *, scale: floa
     """Causal attention of the new tokens over their sequences' pages (whose rows of the new tokens have been written, see rope_append).
 
     q: [tokens, heads, 128] in the pages' type, heads 1, 2, 4 or 8 times the pool's.  Returns out (q's shape and type; not q itself).  A token that sees no position gets zeros;
-    rows that a token does not see (later tokens', slots behind the last position) do not touch its result, whatever they hold.  Equal bits on every run."""
+    rows that a token does not see (later tokens', slots behind the last position) do not touch its result, whatever they hold.  Equal bits on every run.  A wait inside the
+    kernel that gives up leaves NaN in the rows it could not finish and is reported by `batch.pool.status()`."""
     sq = _strides("attention: q", q, batch, batch.dtypes)
     heads = q.shape[1]
     if out is None:
@@ -130,8 +144,8 @@ def attention(batch: PagedBatch, q: torch.Tensor, layer: int = 0, *, scale: floa
     view = batch.view(layer)
     with _on(batch.device):
         space = torch.empty(batch.workspace_bytes(heads), dtype=torch.uint8, device=batch.device)
-        a = _cabi.PagedAttnArgs(q.data_ptr(), out.data_ptr(), sq[0], sq[1], so[0], so[1], heads, scale, space.data_ptr(), space.numel(), None)
-        rc = batch.lib.q3_paged_attn(view, a, _raw_stream(batch.device.index))
+        a = _cabi.PagedAttnArgs(q.data_ptr(), out.data_ptr(), sq[0], sq[1], so[0], so[1], heads, scale, space.data_ptr(), space.numel(), batch._status)
+        rc = batch.lib.q3_paged_attn_limited(view, a, batch.wait_limit_us, _raw_stream(batch.device.index))
     if rc:
         _cabi.check(batch.lib, None, rc, "q3_paged_attn")
     return out

@@ -218,3 +218,14 @@ def test_struct_layouts():
     assert ctypes.sizeof(_cabi.Paged) == 5 * 8 + 4 * 8 + 8 * 4 and _cabi.Paged.type.offset == 100
     assert ctypes.sizeof(_cabi.PagedAttnArgs) == 2 * 8 + 4 * 8 + 8 + 3 * 8
     assert ctypes.sizeof(_cabi.PagedRopeArgs) == 4 * 8 + 8 * 8 + 4 * 8 + 6 * 4
+
+
+def test_bad_limits_and_status_words_are_refused():
+    from qwen3mk import _cabi
+
+    lib, c = _cabi.load(), view()
+    attn = dict(q=1 << 20, out=1 << 21, q_token=2048, q_head=128, out_token=2048, out_head=128, q_heads=16, scale=0.1, workspace=1 << 22, workspace_bytes=1 << 40)
+    for limit, change in ((-1, {}), (5, dict(status=(1 << 20) + 2)), (5, dict(q=None))):
+        assert lib.q3_paged_attn_limited(ctypes.byref(c), ctypes.byref(_cabi.PagedAttnArgs(**{**attn, **change})), limit, None) == _cabi.ERR_INVALID
+        assert lib.q3_last_error(None).startswith(b"q3_paged_attn: ")
+    assert lib.q3_paged_attn_limited(ctypes.byref(view(n_tokens=0)), ctypes.byref(_cabi.PagedAttnArgs(**attn)), 7, None) == 0
