@@ -261,7 +261,7 @@ typedef struct q3_paged {
  * kv_heads times 1, 2, 4 or 8; q head h reads kv head h / (q_heads / kv_heads).  A token that sees no position, or none with a weight (all
  * scores -inf), gets zeros; a row that it does not see does not touch its result, whatever it holds.  fp32 scores, maxima, sums and
  * accumulators; the probabilities enter the product with V in the pages' type.  q and out: element (token, head, dim) at token * _token + head * _head + dim, 16-byte
- * aligned, strides multiples of 8, at least 128; they must not overlap.  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
+ * aligned, strides multiples of 8, at least 128; their rows must not overlap (where their address ranges meet, the token strides have to be the same).  `workspace`: device, at least q3_paged_attn_workspace bytes, 16-byte aligned, for this call alone.
  * `status`: device, 4 words that are 0, or NULL: a wait inside the kernel that gives up reports there as in q3_status (the first one since they were 0) and leaves NaN
  * in the rows it could not finish.  Allocates nothing, no host sync, the same bits on every run. */
 typedef struct q3_paged_attn_args {

@@ -14,6 +14,7 @@
 #include "q3_engine.h"
 #include "q3_gemm_tc.h"
 #include "q3_paged.h"
+#include "q3_rows_meet.h"
 #include "q3_tc_ptx.cuh"
 
 namespace q3 {
@@ -1456,6 +1457,13 @@ extern "C" int q3_paged_attn_limited(const q3_paged* c, const q3_paged_attn_args
     const struct { int64_t stride; int32_t count; } dims[4] = {{p->q_token, c->n_tokens}, {p->out_token, c->n_tokens}, {p->q_head, p->q_heads}, {p->out_head, p->q_heads}};
     for (const auto& d : dims)
         if (d.stride < 0 || d.stride > most || d.stride % 8 || (d.count > 1 && d.stride < HEAD_DIM)) return bad("strides of q and out must be multiples of 8 elements, at least 128");
+    // (rows are stored while others are still read, and q is read again where a result is not finite)
+    const RowSet q_rows{reinterpret_cast<uintptr_t>(p->q), 2 * p->q_token, 2 * p->q_head, c->n_tokens, p->q_heads, 2 * HEAD_DIM};
+    const RowSet o_rows{reinterpret_cast<uintptr_t>(p->out), 2 * p->out_token, 2 * p->out_head, c->n_tokens, p->q_heads, 2 * HEAD_DIM};
+    if (rows_meet_themselves(o_rows)) return bad("rows of out must not overlap");
+    const Meet meet = rows_meet(q_rows, o_rows);
+    if (meet == Meet::Yes) return bad("q and out must not overlap");
+    if (meet == Meet::Unknown) return bad("q and out must not overlap: where their address ranges meet, their token strides must be the same");
     const int64_t need = q3_paged_attn_workspace(c, p->q_heads);
     if (need < 0) return (int)need;
     if (p->workspace_bytes < need) return engine_fail(nullptr, Q3_ERR_INVALID, "%s: workspace holds %lld bytes, %lld needed", who, (long long)p->workspace_bytes, (long long)need);

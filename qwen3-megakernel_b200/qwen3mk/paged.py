@@ -133,7 +133,7 @@ def _strides(what: str, t: torch.Tensor, batch: PagedBatch, dtypes, heads: int |
 def attention(batch: PagedBatch, q: torch.Tensor, layer: int = 0, *, scale: float = HEAD_DIM ** -0.5, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the new tokens over their sequences' pages (whose rows of the new tokens have been written, see rope_append).
 
-    q: [tokens, heads, 128] in the pages' type, heads 1, 2, 4 or 8 times the pool's.  Returns out (q's shape and type; not q itself).  A token that sees no position gets zeros;
+    q: [tokens, heads, 128] in the pages' type, heads 1, 2, 4 or 8 times the pool's.  Returns out (q's shape and type; rows that share no memory with one another or with q's).  A token that sees no position gets zeros;
     rows that a token does not see (later tokens', slots behind the last position) do not touch its result, whatever they hold.  Equal bits on every run.  A wait inside the
     kernel that gives up leaves NaN in the rows it could not finish and is reported by `batch.pool.status()`."""
     sq = _strides("attention: q", q, batch, batch.dtypes)
