@@ -285,7 +285,8 @@ int q3_paged_attn_limited(const q3_paged* c, const q3_paged_attn_args* a, int32_
  *     half layout:  y[i] = n[i] c[i] - n[i + r/2] s[i],   y[i + r/2] = n[i + r/2] c[i] + n[i] s[i],      i < r/2 = rotary_dim / 2
  *     interleaved:  y[2i] = n[2i] c[i] - n[2i + 1] s[i],  y[2i + 1] = n[2i + 1] c[i] + n[2i] s[i]
  * in fp32.  q, k and v: element (token, head, dim) at token * _token + head * _head + dim (they may be slices of one row), 16-byte aligned fp32 or 8-byte
- * aligned bf16 / fp16, strides multiples of 4; q_out in the pages' type, 8-byte aligned, strides multiples of 4 and at least 128, possibly q itself where the types agree.  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
+ * aligned bf16 / fp16, strides multiples of 4; q_out in the pages' type, 8-byte aligned, strides multiples of 4 and at least 128; it is q itself (address, strides and type) or shares no
+ * memory with q, k and v (where address ranges meet, the token strides have to be the same).  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
  * rotary_dim / 2 angles (any scaling of long contexts is in the table).  A token whose position has no row gets NaN (q, k); one without a slot (no page, or
  * kv_len below the number of new tokens) writes no k and v.  `positions`: device [n_tokens] or NULL: rotate by these instead of the tokens' places
  * in their sequences.  q may be NULL (k and v only), and k and v both (q only).  Allocates nothing, no host sync. */

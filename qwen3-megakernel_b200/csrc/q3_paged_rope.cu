@@ -9,6 +9,7 @@
 
 #include "q3_engine.h"
 #include "q3_paged.h"
+#include "q3_rows_meet.h"
 
 namespace q3 {
 
@@ -163,7 +164,6 @@ extern "C" int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* p, voi
     if (p->rows_type != Q3_TYPE_BF16 && p->rows_type != Q3_TYPE_FP16 && p->rows_type != Q3_TYPE_FP32) return bad("rows are fp32, bf16 or fp16");
     if (p->rotary_dim < 0 || p->rotary_dim > HEAD_DIM || p->rotary_dim % 8) return engine_fail(nullptr, Q3_ERR_INVALID, "%s: rotary_dim %d is not a multiple of 8 in 0..128", who, p->rotary_dim);
     if (p->rotary_dim && (!p->rope || p->rope_positions < 1)) return bad("a rotation needs a table");
-    if (!(p->eps >= 0.f)) return bad("eps must not be negative");
     const int esize = p->rows_type == Q3_TYPE_FP32 ? 4 : 2;
     const uintptr_t in = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
     if (in & (esize == 4 ? 15 : 7)) return bad("fp32 rows must be 16-byte aligned, 16-bit rows 8-byte aligned");
@@ -174,6 +174,18 @@ extern "C" int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* p, voi
     for (int64_t s : {p->q_token, p->q_head, p->k_token, p->k_head, p->v_token, p->v_head, p->out_token, p->out_head})
         if (s < 0 || s > most || s % 4) return bad("strides must be multiples of 4 elements, not negative");
     if (p->q && ((c->n_tokens > 1 && p->out_token < HEAD_DIM) || (p->q_heads > 1 && p->out_head < HEAD_DIM))) return bad("rows of q_out must not overlap: strides of at least 128");
+    if (p->q) {
+        // a warp stores a token's rows while others still read theirs: q_out is q itself, row by row, or shares nothing with what is read
+        const int width = HEAD_DIM * esize;
+        auto rows = [&](const void* at, int64_t token, int64_t head, int heads) { return RowSet{reinterpret_cast<uintptr_t>(at), token * esize, head * esize, c->n_tokens, heads, width}; };
+        const RowSet out{reinterpret_cast<uintptr_t>(p->q_out), 2 * p->out_token, 2 * p->out_head, c->n_tokens, p->q_heads, 2 * HEAD_DIM};
+        if (rows_meet_themselves(out)) return bad("rows of q_out must not overlap");
+        const bool in_place = p->q_out == p->q && p->rows_type == c->type && (c->n_tokens == 1 || p->out_token == p->q_token) && (p->q_heads == 1 || p->out_head == p->q_head);
+        if ((!in_place && rows_meet(rows(p->q, p->q_token, p->q_head, p->q_heads), out) != Meet::No) ||
+            (p->k && (rows_meet(rows(p->k, p->k_token, p->k_head, c->kv_heads), out) != Meet::No || rows_meet(rows(p->v, p->v_token, p->v_head, c->kv_heads), out) != Meet::No)))
+            return bad("q_out must not overlap k, v or q, unless it is q itself in the pages' type (where address ranges meet, token strides must be the same)");
+    }
+    if (!(p->eps >= 0.f)) return bad("eps must not be negative");
     PagedRopeArgs a{};
     a.c = paged_view(c);
     a.sh.heads = c->kv_heads; a.sh.batch = c->batch; a.sh.n_tokens = c->n_tokens; a.sh.most_keys = c->table_pages * c->page_size;

@@ -155,7 +155,7 @@ def rope_append(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Te
                 k_gain: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, positions: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """The new tokens' rows: RMS norm of every q and k head (where a gain, bf16 [128], is given), rotary embedding, k and v into the pages.  Returns q's rows in the
-    pages' type (`out` when given: q itself where the types agree, say), as `attention` reads them.
+    pages' type (`out` when given: q itself where the types agree, or rows that share no memory with q, k and v), as `attention` reads them.
 
     q [tokens, heads, 128], k and v [tokens, kv_heads, 128]: fp32, bf16 or fp16, all three alike; slices of one projection's rows serve.  rope: fp32
     [positions, rotary_dim], contiguous, a row the cosines and then the sines (`rope_table`); its width says how many dims of a head are rotated (a multiple of 8

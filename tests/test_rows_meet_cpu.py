@@ -80,4 +80,29 @@ def test_attention_takes_rows_that_lie_beside_one_another(change):
 
     lib = _cabi.load()
     lib.q3_paged_attn(ctypes.byref(view()), ctypes.byref(_cabi.PagedAttnArgs(**{**ATTN, **change})), None)
-    assert b"overlap" not in lib.q3_last_error(None) and b"strides" not in lib.q3_last_error(None)
+    assert b"workspace" in lib.q3_last_error(None)
+
+
+ROPE = dict(q=1 << 24, k=(1 << 24) + 16 * 256, v=(1 << 24) + 24 * 256, q_out=1 << 26, q_token=4096, q_head=128, k_token=4096, k_head=128, v_token=4096, v_head=128, out_token=2048, out_head=128,
+            q_heads=16, rows_type=0, rope_positions=0, rotary_dim=0, eps=-1.0)      # the last one is refused behind the overlaps' turn: nothing is launched where a GPU is
+IN_PLACE = dict(q_out=1 << 24, out_token=4096)
+
+
+@pytest.mark.parametrize("change", [dict(q_out=1 << 24), dict(q_out=(1 << 24) + 256, out_token=4096), dict(q_out=(1 << 24) + 16 * 256, out_token=4096), dict(q_out=(1 << 24) + 24 * 256 - 8, out_token=4096),
+                                    {**IN_PLACE, "rows_type": 1}, {**IN_PLACE, "rows_type": 2}, {**IN_PLACE, "q_head": 256, "q_token": 8192}, dict(out_token=256)])
+def test_rope_refuses_rows_that_overlap(change):
+    from qwen3mk import _cabi
+
+    lib = _cabi.load()
+    assert lib.q3_paged_rope(ctypes.byref(view()), ctypes.byref(_cabi.PagedRopeArgs(**{**ROPE, **change})), None) == _cabi.ERR_INVALID
+    assert b"overlap" in lib.q3_last_error(None)
+
+
+@pytest.mark.parametrize("change", [{}, IN_PLACE, dict(q_out=(1 << 24) - 3 * 8192), dict(q_out=(1 << 24) + 3 * 8192), dict(q_token=8192, k_token=8192, v_token=8192, q_out=(1 << 24) + 8192, out_token=8192),
+                                    {**IN_PLACE, "k": None, "v": None}, dict(q_out=(1 << 24) + 8192, q_token=0, out_token=4096)])      # (the last: one row of q for all tokens)
+def test_rope_takes_rows_that_lie_beside_one_another(change):
+    from qwen3mk import _cabi
+
+    lib = _cabi.load()
+    assert lib.q3_paged_rope(ctypes.byref(view()), ctypes.byref(_cabi.PagedRopeArgs(**{**ROPE, **change})), None) == _cabi.ERR_INVALID
+    assert b"eps" in lib.q3_last_error(None)
