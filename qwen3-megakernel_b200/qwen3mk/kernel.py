@@ -162,6 +162,7 @@ class Megakernel:
         _cabi.check(self.lib, None, rc, "q3_create")
         self.handle = h
         self.rope = rope_rows(int(max_positions), self.device)
+        self._ropes = [self.rope]
         _cabi.check(self.lib, h, self.lib.q3_set_rope(h, self.rope.data_ptr(), self.rope.shape[0]), "q3_set_rope")
         g, t, s = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
         self.lib.q3_grid_info(h, ctypes.byref(g), ctypes.byref(t), ctypes.byref(s))
@@ -225,11 +226,14 @@ class Megakernel:
 
     def set_rope(self, table: torch.Tensor) -> None:
         """Rotary table of every later call: fp32 [positions, 128] on the engine's device (`paged.rope_table`, scaled for long contexts, say).  Borrowed; a bound
-        launch follows it with its next launch."""
+        launch follows it with its next launch.  A call that was captured into a CUDA graph keeps the table that it was captured with (the engine keeps every table it has had
+        alive as long as itself): capture it again to follow."""
         if table.dim() != 2 or table.shape[1] != HEAD_DIM or table.dtype != torch.float32 or not table.is_contiguous() or table.device != self.device:
             raise ValueError(f"set_rope: expected a contiguous float32 [positions, {HEAD_DIM}] on {self.device}, got {table.dtype} {tuple(table.shape)} on {table.device}")
         _cabi.check(self.lib, self.handle, self.lib.q3_set_rope(self.handle, table.data_ptr(), table.shape[0]), "q3_set_rope")
         self.rope = table
+        if not any(t is table for t in self._ropes):
+            self._ropes.append(table)
 
     def check_inputs(self, inputs: dict) -> None:
         """Raise ValueError unless every input is a contiguous CUDA tensor of the expected shape and dtype."""
