@@ -23,13 +23,13 @@ import math
 import torch
 
 from . import _cabi
+from ._stream import raw_stream as _raw_stream
 
 HEAD_DIM = 128
 ROPE_THETA = 1e6
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NO_SWITCH = contextlib.nullcontext()
 _current_device = torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(device).cuda_stream without the Stream object (2.1 us of a call of 17)
 
 
 def _on(device: torch.device):

@@ -14,6 +14,7 @@ import contextlib
 import torch
 
 from . import _cabi
+from ._stream import raw_stream as _raw_stream
 
 
 def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, *, generator: torch.Generator | None = None,
@@ -57,7 +58,6 @@ def sample_reference(logits: torch.Tensor, temperature: float, top_k: int, u: to
 
 
 _NO_SWITCH = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(device).cuda_stream without the Stream object
 _FILTERS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
 

@@ -264,3 +264,20 @@ def test_row_sums_of_the_persistent_kernel_end_before_the_query_heads(many):
     heads = re.search(r"float\* q_s = ([^;]+);", code)
     begin, words = eval(sums.group(1 if many else 2), names), 512 * names["NB"]
     assert begin + words <= eval(heads.group(1), names), (begin, words)
+
+
+def test_modules_import_with_a_torch_without_cuda():
+    """Such a build lacks the private names of torch's CUDA part; the rules of sampling and the rotary tables run on the CPU all the same."""
+    import subprocess
+    import sys
+
+    program = """
+import torch
+del torch._C._cuda_getCurrentRawStream
+from qwen3mk import paged, sampling
+assert int(sampling.sample_reference(torch.tensor([[0.0, 5.0, 1.0]]), 1.0, 1, torch.tensor([0.5]))) == 1
+assert paged.rope_table(4, "cpu").shape == (4, 128)
+print("ok")
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, env={**__import__("os").environ, "PYTHONPATH": str(ROOT / "qwen3-megakernel_b200")})
+    assert done.stdout.strip() == "ok", done.stderr
