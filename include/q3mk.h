@@ -316,7 +316,7 @@ int q3_paged_rope(const q3_paged* c, const q3_paged_rope_args* a, void* stream);
 typedef struct q3_extend_args {
     const q3_paged* pages;
     int64_t layer_stride;
-    const int64_t* ids;          /* device [n_tokens]                 */
+    const int64_t* ids;          /* device [n_tokens]; those of rows behind q_start[batch] may be anything */
     float* logits;               /* device [batch][vocab] fp32, or NULL */
     int64_t* next_token;         /* device [batch]                    */
     void* workspace;

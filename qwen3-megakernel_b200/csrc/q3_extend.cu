@@ -102,7 +102,7 @@ extern "C" int q3_extend(q3_engine* e, const q3_extend_args* a, void* stream) {
     const uint32_t box = (uint32_t)prompt_box_rows(T);
     if (!tc_make_map(&m_xn, xn, 0, T, HIDDEN, 1, box) || !tc_make_map(&m_hid, hid, 0, T, INTER, 1, box) || !tc_make_map(&m_attn, attn, 0, T, Q_DIM, 1, box))
         return fail(e, Q3_ERR_CUDA, "q3_extend: a tensor map could not be encoded");
-    LAUNCH(1, launch_prompt_embed(reinterpret_cast<const long long*>(a->ids), bf(w.embed), V, e->x, bf(w.ln1), xn, ssq, T, e->status, T, st));
+    LAUNCH(1, launch_prompt_embed(reinterpret_cast<const long long*>(a->ids), bf(w.embed), V, e->x, bf(w.ln1), xn, ssq, T, e->status, T, st, pg.q_start, B));
     for (int l = 0; l < L; ++l) {
         PromptGemmCall c{};
         c.T = T; c.ssq = ssq; c.ssq_ld = T; c.parts = &parts; c.status = e->status;

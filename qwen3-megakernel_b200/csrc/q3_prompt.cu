@@ -858,13 +858,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prompt_pair_kernel(const __grid
 // ---- embedding gather: a block per token -------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) prompt_embed_kernel(const long long* __restrict__ ids, const bf16_raw* __restrict__ embed, int vocab, float* __restrict__ x,
                                                            const bf16_raw* __restrict__ gain, bf16_raw* __restrict__ xn, float* __restrict__ ssq, int ssq_ld,
-                                                           uint32_t* status) {
+                                                           uint32_t* status, const int* q_start, int batch) {
     pdl_launch();
     pdl_wait();
     const int b = blockIdx.x, tid = threadIdx.x;
     long long t = ids[b];
     if (t < 0 || t >= vocab) {
-        if (tid == 0) report(status, ST_BAD_TOKEN, 0, (uint32_t)t);
+        if (tid == 0 && (q_start == nullptr || (b >= q_start[0] && b < q_start[batch]))) report(status, ST_BAD_TOKEN, 0, (uint32_t)t);
         t = 0;
     }
     const float4 v = pr_unpack4(reinterpret_cast<const uint2*>(embed + (size_t)t * HIDDEN)[tid]), g = pr_unpack4(reinterpret_cast<const uint2*>(gain)[tid]);
@@ -877,8 +877,8 @@ __global__ void __launch_bounds__(256) prompt_embed_kernel(const long long* __re
 }
 
 cudaError_t launch_prompt_embed(const long long* ids, const bf16_raw* embed, int vocab, float* x, const bf16_raw* gain, bf16_raw* xn, float* ssq, int ssq_ld,
-                                uint32_t* status, int T, cudaStream_t st) {
-    return launch_chain(prompt_embed_kernel, dim3(T), dim3(256), 0, st, ids, embed, vocab, x, gain, xn, ssq, ssq_ld, status);
+                                uint32_t* status, int T, cudaStream_t st, const int* q_start, int batch) {
+    return launch_chain(prompt_embed_kernel, dim3(T), dim3(256), 0, st, ids, embed, vocab, x, gain, xn, ssq, ssq_ld, status, q_start, batch);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------

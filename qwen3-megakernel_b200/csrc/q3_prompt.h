@@ -43,8 +43,9 @@ inline int prompt_box_rows(int T) { return T < 128 ? (T + 15) / 16 * 16 : 128; }
 cudaError_t launch_prompt_gemm(const PromptGemmCall& c, cudaStream_t st);
 
 // x[t] = embed[ids[t]], its plane times `gain`, its partial sums of squares; a bad id is reported and read as 0
+// q_start given: rows before q_start[0] and from q_start[batch] on are padding, and what stands in their ids is nobody's mistake (they are embedded as token 0)
 cudaError_t launch_prompt_embed(const long long* ids, const bf16_raw* embed, int vocab, float* x, const bf16_raw* gain, bf16_raw* xn, float* ssq, int ssq_ld,
-                                uint32_t* status, int T, cudaStream_t st);
+                                uint32_t* status, int T, cudaStream_t st, const int* q_start = nullptr, int batch = 0);
 
 // causal attention of a prompt of T >= 1 tokens: q planes and caches as above -> bf16 plane [T][2048]
 cudaError_t launch_prefill_attn_tc(const ::CUtensorMap_st& q_hi, const ::CUtensorMap_st& q_lo, const ::CUtensorMap_st& k, const ::CUtensorMap_st& v, int layer,

@@ -312,7 +312,8 @@ class Megakernel:
 
     def extend(self, weights: dict, ids: torch.Tensor, batch, *, want_logits: bool = True) -> dict:
         """New tokens of many sequences over a pool of cache pages (`paged.PagePool`, `paged.PagedBatch`): prompts, chunks of prompts, known turns and single tokens
-        side by side.  ids: int64 [batch.tokens] on the device, sequence after sequence; batch.kv_len counts them already.  Writes their K and V rows into the pages and
+        side by side.  ids: int64 [batch.tokens] on the device, sequence after sequence (behind the last sequence's, where batch.tokens is more than
+        they are, anything); batch.kv_len counts them already.  Writes their K and V rows into the pages and
         returns `logits` [B, vocab] (None without want_logits) and `next_token` [B] of every sequence's last new token, fresh tensors.  Enqueues on the current stream
         without synchronising; `status()` reports descriptors that do not fit.
 
