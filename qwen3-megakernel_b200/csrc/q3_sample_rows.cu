@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(SR_THREADS, 1) sample_rows_kernel(const Sample
     const int i0 = run_start(warp), i1 = run_start(warp + 1);
     const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
     // (below 1e-36 the factor and its products would leave fp32's range; words that differ by more than 1e-34 have weights of 0 or 1 there, too)
-    const float T0 = a.temperature ? a.temperature[row_id] : a.temperature1, T = T0 > 0.f ? fmaxf(T0, 1e-36f) : T0, u = a.uniform ? a.uniform[row_id] : 0.f;
+    const float T0 = a.temperature ? a.temperature[row_id] : a.temperature1, T = T0 > 0.f ? fmaxf(T0, 1e-36f) : T0, u = a.uniform[row_id];
     const int k = a.top_k ? a.top_k[row_id] : a.top_k1;
     float p = a.top_p ? a.top_p[row_id] : a.top_p1, min_p = a.min_p ? a.min_p[row_id] : a.min_p1;
     if (!(p < 1.f)) p = 1.f;
