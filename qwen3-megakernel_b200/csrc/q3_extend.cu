@@ -76,13 +76,13 @@ extern "C" int q3_extend(q3_engine* e, const q3_extend_args* a, void* stream) {
     if (T < 1 || T > e->cap) return fail(e, Q3_ERR_INVALID, "q3_extend: %d tokens outside 1..%d (the larger of max_tokens and max_batch)", T, e->cap);
     if (B > e->cfg.max_batch) return fail(e, Q3_ERR_INVALID, "q3_extend: %d sequences exceed max_batch %d", B, e->cfg.max_batch);
     if (!a->ids || !a->next_token) return fail(e, Q3_ERR_INVALID, "q3_extend: ids and next_token are required");
+    const cudaError_t dev = cudaSetDevice(e->device);                 // (the workspace goes by this device's SMs)
+    if (dev != cudaSuccess) return fail(e, Q3_ERR_CUDA, "q3_extend: %s", cudaGetErrorString(dev));
     const int64_t need = q3_paged_attn_workspace(&pg, Q_HEADS);
     if (need < 0) return fail(e, (int)need, "q3_extend: %s", q3_last_error(nullptr));
     if (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))
         return fail(e, Q3_ERR_INVALID, "q3_extend: workspace holds %lld bytes, %lld needed, 16-byte aligned", (long long)a->workspace_bytes, (long long)need);
     cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t dev = cudaSetDevice(e->device);
-    if (dev != cudaSuccess) return fail(e, Q3_ERR_CUDA, "q3_extend: %s", cudaGetErrorString(dev));
 #define LAUNCH(n, call)                                                                                \
     do {                                                                                               \
         cudaError_t err__ = (call);                                                                    \
