@@ -596,7 +596,8 @@ struct PtGroup {
         sync();
     }
 };
-constexpr uint32_t PT_AGAIN = 0x7fff7fffu;                    // what a finished row begins with that is to be done again (finished rows hold no NaN)
+// What a row begins with that is to be done again: no number, and not the NaN that a conversion gives.  In a partial result: a maximum that is NaN with a sum of 0.
+constexpr uint32_t PT_AGAIN = 0x7fff7ffeu;
 
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -1093,11 +1094,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
                 }
                 const float2 odd2 = pt_unpair(odd);
                 bad = (bad || odd2.x != 0.f || odd2.y != 0.f) && row < d.rows;
-                if (bad) {                           // marked, and done again when nobody waits any more
-                    if (whole) *reinterpret_cast<uint32_t*>(o_row) = PT_AGAIN;
-                    else reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(NAN, NAN);
-                    s_any = 1;
-                }
+                // A sum that is NaN has a seen score that is NaN or infinite in it (what is hidden is -inf before the exponential): the row is NaN, and once more would not change it.
+                // All others are marked, and done again when nobody waits any more.
+                const bool spoiled = sum != sum;
+                if (bad && !spoiled) s_any = 1;
+                if (bad && whole && !spoiled) *reinterpret_cast<uint32_t*>(o_row) = PT_AGAIN;
+                if (bad && !whole) reinterpret_cast<float2*>(parts + 128 * HEAD_DIM)[row] = make_float2(NAN, spoiled ? NAN : 0.f);
             }
             if (n > 0) {
                 ++n_q;
@@ -1155,7 +1157,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             float2* const stats = reinterpret_cast<float2*>(parts + 128 * HEAD_DIM);
             if (warp < 4) {
                 bool bad = tid < keys.rows;
-                if (bad) bad = whole ? *reinterpret_cast<const uint32_t*>(pg_o_row(a, seg, tid)) == PT_AGAIN : stats[tid].x != stats[tid].x;
+                if (bad) bad = whole ? *reinterpret_cast<const uint32_t*>(pg_o_row(a, seg, tid)) == PT_AGAIN : stats[tid].x != stats[tid].x && stats[tid].y == 0.f;
                 const unsigned again = __ballot_sync(0xffffffffu, bad);
                 if (lane == 0) s_again[warp] = again;
             }

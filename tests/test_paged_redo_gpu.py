@@ -120,3 +120,36 @@ def test_pages_that_are_gone_cost_nothing(dtype, kept):
     check(out, q, rows, [new], [n], there=there)
     less = median_us(lambda: paged.attention(batch, q))
     assert less < 2 * whole, f"{less:.0f} us without {gone} pages, {whole:.0f} us with them"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,n", [(64, 33064), (300, 300), (40, 170)])
+def test_rows_that_are_no_numbers_cost_nothing(dtype, new, n):
+    """Queries that are NaN (positions behind a rotary table's end, say) and a K row that is: their rows are NaN, the others right, and nothing is done again for them
+    but where an infinite V row asks for it as well."""
+    from qwen3mk import paged
+
+    g = torch.Generator().manual_seed(205)
+    pool, table, rows = make_pool(g, [n, 50], 64, 8, dtype)
+    q = torch.randn(new + 20, 16, D, generator=g).to(dtype).cuda()
+    batch = describe(pool, table, [new, 20], [n, 50])
+    plain = median_us(lambda: paged.attention(batch, q))
+    broken = q.clone()
+    broken[:new:2] = float("nan")
+    out = paged.attention(batch, broken)
+    lost = torch.zeros(new + 20, dtype=torch.bool, device="cuda")
+    lost[:new:2] = True
+    assert torch.isnan(out[lost]).all()
+    kept = ~lost
+    want = paged.attention(batch, q)
+    check(want, q, rows, [new, 20], [n, 50])
+    assert torch.equal(out[kept], want[kept])
+    slow = median_us(lambda: paged.attention(batch, broken))
+    assert slow < 2 * plain + 20, f"{slow:.0f} us with NaN, {plain:.0f} us without"
+    # a K row that every token of the first sequence sees, and an infinite V row that the last one sees
+    at, s = slot(pool, table, 0, 0)
+    pool.k[0, at, s, 2] = rows[0][0][0, 2] = float("nan")
+    at, s = slot(pool, table, 0, n - 1)
+    pool.v[0, at, s, 2, 9] = rows[0][1][n - 1, 2, 9] = float("inf")
+    pool.v[0, at, s, 4, 9] = rows[0][1][n - 1, 4, 9] = float("inf")
+    check(paged.attention(batch, q), q, rows, [new, 20], [n, 50])
