@@ -484,12 +484,14 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(const __grid_
 // above 2^-100 though it sees keys) is seen by its sum: both are marked, and done again row by row once the block's run is over and nobody waits any more.
 // fp16: P must not leave [2^-24, 2^16), so m follows a group's maximum, and its O is rescaled when a score exceeds m by 2^8; two S and two O.
 // P is rounded to the pages' type and its sum is that of the rounded values: where few keys hold a row's weight their roundings leave the quotient.  2048 tokens
-// behind 8192: 2.3e-3 off, 1.7e-3 of it the output's own rounding (P truncated, as fast: 2.4e-3, and 2.6e-3 with short sequences).
+// behind 8192: 2.3e-3 off, 1.7e-3 of it the output's own rounding (P truncated, as fast: 2.4e-3, and 2.6e-3 with short sequences; a second plane of P would be a third product, 1700 clocks a tile
+// for products alone).
 //
-// Measured: 2048 tokens behind 8192 143 us, 1.08 PFLOP/s of the 1.64 that a large product reaches; 1650 clocks a tile, of which the special-function pipe has 1024 (an exponential a score),
+// Measured: 2048 tokens behind 8192 143 to 168 us from box to box (the clock that the power cap leaves), 0.92 to 1.08 PFLOP/s of the 1.64 that a large product reaches, fp16 205 where bf16
+// takes 147; 1650 clocks a tile, of which the special-function pipe has 1024 (an exponential a score),
 // the products 1150, the rest are hand-offs.  (Steps: K and V loaded by warps of their own, a thread a row 247 -> 211; one O, scores two tiles ahead 208 -> 178;
 // segments worked out ahead, one lane that looks for a group 166 -> 149; masks as bits, O free before its rows are stored 145 -> 143.  A third group of warps that only writes: 128 registers a thread, 153.)  Few rows: 8 sequences of 13 tokens behind up
-// to 5000, fp16, 38 us; the pages at 6.7 TB/s in the steady state (15.9), the rest start, segment ends and join.
+// to 5000, fp16, 37 to 39 us; the pages at 6.7 TB/s in the steady state (15.9), start, segment ends and join 11, the rest not accounted for.
 //
 // A wait that gives up lets every later one give up at once (those in which the softmax warps meet are waits like the others); the block then drains what is under way and
 // leaves NaN in all rows of its run.
