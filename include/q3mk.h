@@ -203,7 +203,7 @@ int q3_sample(const float* logits, int32_t batch, int32_t vocab, float temperatu
  * likely word is always kept); return the first index whose inclusive sum of kept weights exceeds uniform[row] * total, in index order.  The
  * arrays (device, [batch]) may be NULL: then the number beside them serves all rows.  temperature <= 0, top_k == 1 or min_p > 1, and rows that have no draw (a NaN
  * or an infinite maximum among the logits, a uniform number outside [0, 1)) give the arg-max (ties -> lowest index).  Logits of -inf are never
- * drawn; values that no parameter may have (a NaN, a negative top_k) switch that filter off, a temperature that is NaN gives the arg-max.  Row r begins at logits + r * row_stride.  The same
+ * drawn; values that no parameter may have (a NaN, a negative top_k or min_p) switch that filter off, a negative top_p is 0, a temperature that is NaN gives the arg-max.  Row r begins at logits + r * row_stride.  The same
  * logits and numbers draw the same words on every run.  Allocates nothing, no host sync.  q3_sample, with one temperature and one top_k for all rows, sums in fp32. */
 typedef struct q3_sample_rows_args {
     const float* logits;         /* device [batch][row_stride] fp32, vocab words a row */

@@ -52,10 +52,14 @@ class PagePool:
         self.device, self.dtype = k.device, k.dtype
         self._status = torch.zeros(4, dtype=torch.int32, device=k.device)      # what `attention` reports of a wait that gave up
 
-    def status(self, stream: torch.cuda.Stream | None = None) -> list[int]:
-        """Synchronise the (current) stream and read the status words of `attention` over this pool; raises RuntimeError, and clears them, if a wait inside a kernel gave
+    def status(self, stream=None) -> list[int]:
+        """Synchronise a stream (the current one, a Stream or its address) and read the status words of `attention` over this pool; raises RuntimeError, and clears them, if a wait inside a kernel gave
         up: rows of that call are NaN.  (`Megakernel.extend` reports to `Megakernel.status`.)"""
-        (torch.cuda.current_stream(self.device) if stream is None else stream).synchronize()
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        elif isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=self.device)
+        stream.synchronize()
         words = self._status.tolist()
         if words[0]:
             self._status.zero_()
