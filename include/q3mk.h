@@ -231,7 +231,8 @@ int q3_sample_rows(const q3_sample_rows_args* a, void* stream);
  * kv_len[b] - (kv_len[b] - new) positions, i.e. its token i stands at position kv_len[b] - new + i.  A sequence may have no new token; rows
  * behind q_start[batch] belong to nobody and are left as they were.  All descriptors lie in device memory and are read
  * when the call runs: a captured call may be replayed with others.  What they say is cut down to what there is
- * (n_tokens rows, table_pages * page_size positions), so that no value reads or writes out of bounds.
+ * (n_tokens rows, table_pages * page_size positions: a longer sequence is attended as if it ended there, and its tokens behind that are not stored), so that no
+ * value reads or writes out of bounds.
  * Strides are in elements; the 128 elements of a head are contiguous, pages 16-byte aligned and strides multiples of 8 that are at
  * least 128, the same for K and V. */
 #define Q3_TYPE_BF16 0
@@ -287,8 +288,8 @@ int q3_paged_attn_limited(const q3_paged* c, const q3_paged_attn_args* a, int32_
  * in fp32.  q, k and v: element (token, head, dim) at token * _token + head * _head + dim (they may be slices of one row), 16-byte aligned fp32 or 8-byte
  * aligned bf16 / fp16, strides multiples of 4; q_out in the pages' type, 8-byte aligned, strides multiples of 4 and at least 128; it is q itself (address, strides and type) or shares no
  * memory with q, k and v (where address ranges meet, the token strides have to be the same).  `rope`: fp32 [rope_positions][rotary_dim], a row is the cosines and then the sines of
- * rotary_dim / 2 angles (any scaling of long contexts is in the table).  A token whose position has no row gets NaN (q, k); one without a slot (no page, or
- * kv_len below the number of new tokens) writes no k and v.  `positions`: device [n_tokens] or NULL: rotate by these instead of the tokens' places
+ * rotary_dim / 2 angles (any scaling of long contexts is in the table).  A token whose position has no row gets NaN (q, k); one without a slot (no page, a position
+ * behind the page table's row, or kv_len below the number of new tokens) writes no k and v.  `positions`: device [n_tokens] or NULL: rotate by these instead of the tokens' places
  * in their sequences.  q may be NULL (k and v only), and k and v both (q only).  Allocates nothing, no host sync. */
 typedef struct q3_paged_rope_args {
     const void *q, *k, *v;

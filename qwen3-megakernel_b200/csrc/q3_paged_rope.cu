@@ -77,8 +77,10 @@ __global__ void __launch_bounds__(RP_THREADS) paged_rope_kernel(const PagedRopeA
     if (b >= a.sh.batch) return;
     const PgSeq s = pg_seq(a.sh, a.c.q_start, a.c.kv_len, b);
     if (t < s.q0 || t >= s.q0 + s.q) return;          // (before the first sequence)
-    const int place = s.kv - s.q + (int)(t - s.q0);
-    const int page = place >= 0 && a.kv_rows ? pg_page(a.c, b, place) : -1;
+    // (by kv_len as it stands: a sequence that has outgrown its page table has no slot for its last tokens, and must not write over earlier ones)
+    const long long stands = (long long)max(a.c.kv_len[b], 0) - s.q + (t - s.q0);
+    const int place = (int)min(stands, 0x7fffffffll);
+    const int page = place >= 0 && place < a.sh.most_keys && a.kv_rows ? pg_page(a.c, b, place) : -1;
     const int pos = a.positions ? a.positions[t] : place;
     const long long slot = page < 0 ? -1 : pg_offset(a.c, page, place & ((1 << a.c.page_log) - 1), 0);
     // this lane's cosines and sines: of d0 .. d0 + 3 and their partners d1 .., or of two pairs in each; what is not rotated is multiplied by one

@@ -6,7 +6,7 @@
   o = attention(batch, q, layer)                                   the new tokens attend their sequences' pages
 
 Position p of sequence b is slot p % page_size of page page_table[b, p // page_size].  An entry outside the pool (-1, say) is a page that is
-not there: nothing is written to it and its positions are not attended.  The new tokens' rows lie one sequence after the other, sequence b's from
+not there: nothing is written to it and its positions are not attended; so are positions behind the table's row.  The new tokens' rows lie one sequence after the other, sequence b's from
 q_start[b] to q_start[b + 1]; they are its last positions of kv_len[b], which counts them.  One new token is a decode step, many are a prompt or
 a chunk of one, none is a sequence that sits this call out.
 
